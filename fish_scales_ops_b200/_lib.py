@@ -51,6 +51,14 @@ SIGNATURES = {
     "fso_ep_dispatch_push": [_c_p] * 12 + [_c_i64, _c_i64, _c_i64, _c_i64, _c_p],
     "fso_moe_gather_rows": [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p],
     "fso_moe_combine_scatter": [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_p],
+    "fso_gated_linear_saved_cols": [_c_i64, ctypes.POINTER(_c_i64)],
+    "fso_gated_linear_ws_bytes": [_c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64)],
+    "fso_gated_linear": [_c_p, _c_i64] + [_c_p] * 4 + [_c_i64] * 5 + [_c_p, _c_i64, _c_p],
+    "fso_gated_linear_backward_ws_bytes": [_c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64)],
+    "fso_gated_linear_backward": [_c_p, _c_i64, _c_p, _c_i64] + [_c_p] * 5 + [_c_i64] * 5 + [_c_p, _c_i64, _c_p],
+    "fso_int4_quantize": [_c_p] * 4 + [_c_i64] * 5 + [_c_p],
+    "fso_int4_linear": [_c_p, _c_i64] + [_c_p] * 5 + [_c_i64] * 6 + [_c_p],
+    "fso_int4_gated_linear": [_c_p, _c_i64] + [_c_p] * 4 + [_c_i64] * 7 + [_c_p],
 }
 
 

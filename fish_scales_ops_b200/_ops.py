@@ -331,3 +331,101 @@ def moe_combine_scatter(dn, slot, topk_w, recv_off, back_base, peer_back, world:
 
 def device_status() -> int:
     return _lib.device_status()
+
+
+# ------------------------------------------------------------------------------- 16-bit gated projection, 4-bit weights
+
+GATE_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+DTYPES_16 = {torch.bfloat16: 0, torch.float16: 1}
+_SCALE_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def rows_in_place(x: torch.Tensor):
+    """(x, elements between its rows) for a 16-bit [T, K] that the kernels can read where it lies: rows dense, their
+    starts on 16-byte boundaries and no two rows overlapping; a copy of it otherwise."""
+    t, k = x.shape
+    ld = x.stride(0) if t > 1 else k
+    if (x.stride(1) == 1 or k == 1) and ld >= k and ld % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x, ld
+    return x.clone(memory_format=torch.contiguous_format), k
+
+
+def gated_linear(x, gate_up, activation: int, save: bool):
+    """x [T, K], gate_up [2I, K] -> (h [T, I], saved upper 16 bits, saved lower 8 bits); the saved arrays are empty
+    without ``save``."""
+    t, k = int(x.shape[0]), int(x.shape[1])
+    inter = int(gate_up.shape[0]) // 2
+    with on_device(x.device):
+        h = torch.empty((t, inter), dtype=x.dtype, device=x.device)
+        cols = 2 * _align(inter, 16) if save else 0
+        hi = torch.empty((t, cols), dtype=torch.int16, device=x.device)
+        lo = torch.empty((t, cols), dtype=torch.uint8, device=x.device)
+        if t > 0:
+            x, ldx = rows_in_place(x)
+            need = ctypes.c_int64(0)
+            check(lib().fso_gated_linear_ws_bytes(t, k, inter, ctypes.byref(need)), "fso_gated_linear_ws_bytes")
+            ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device) if need.value else None
+            check(lib().fso_gated_linear(ptr(x), ldx, ptr(gate_up), ptr(h), ptr(hi) if save else None,
+                                         ptr(lo) if save else None, t, k, inter, DTYPES_16[x.dtype], activation, ptr(ws),
+                                         need.value, stream_ptr()), "fso_gated_linear")
+    return h, hi, lo
+
+
+def gated_linear_backward(dh, x, gate_up, hi, lo, activation: int, need_x: bool, need_w: bool):
+    """(dx [T, K] or empty, dgate_up [2I, K] or empty) for dh [T, I]."""
+    t, k = int(x.shape[0]), int(x.shape[1])
+    inter = int(gate_up.shape[0]) // 2
+    with on_device(x.device):
+        dx = torch.empty((t if need_x else 0, k), dtype=x.dtype, device=x.device)
+        dw = (torch.empty if t > 0 else torch.zeros)((2 * inter if need_w else 0, k), dtype=x.dtype, device=x.device)
+        if t > 0 and (need_x or need_w):
+            x, ldx = rows_in_place(x)
+            if (inter > 1 and dh.stride(1) != 1) or (t > 1 and dh.stride(0) < inter):
+                dh = dh.contiguous()
+            need = ctypes.c_int64(0)
+            check(lib().fso_gated_linear_backward_ws_bytes(t, k, inter, ctypes.byref(need)),
+                  "fso_gated_linear_backward_ws_bytes")
+            ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device)
+            check(lib().fso_gated_linear_backward(ptr(dh), dh.stride(0) if t > 1 else inter, ptr(x), ldx, ptr(gate_up),
+                                                  ptr(hi), ptr(lo), ptr(dx) if need_x else None,
+                                                  ptr(dw) if need_w else None, t, k, inter, DTYPES_16[x.dtype], activation,
+                                                  ptr(ws), need.value, stream_ptr()), "fso_gated_linear_backward")
+    return dx, dw
+
+
+def int4_linear(x, codes, scale, zero, bias):
+    """x [M, K] and a 4-bit weight of N rows -> y [M, N]."""
+    m, k, n = int(x.shape[0]), int(x.shape[1]), int(codes.shape[0])
+    with on_device(x.device):
+        y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        if m > 0:
+            x, ldx = rows_in_place(x)
+            check(lib().fso_int4_linear(ptr(x), ldx, ptr(codes), ptr(scale), ptr(zero), ptr(bias), ptr(y), m, n, k,
+                                        k // int(scale.shape[1]), DTYPES_16[x.dtype], _SCALE_DTYPES[scale.dtype],
+                                        stream_ptr()), "fso_int4_linear")
+    return y
+
+
+def int4_gated_linear(x, codes, scale, zero, activation: int):
+    """x [M, K] and a 4-bit gate_up of 2I rows -> h [M, I]."""
+    m, k, inter = int(x.shape[0]), int(x.shape[1]), int(codes.shape[0]) // 2
+    with on_device(x.device):
+        h = torch.empty((m, inter), dtype=x.dtype, device=x.device)
+        if m > 0:
+            x, ldx = rows_in_place(x)
+            check(lib().fso_int4_gated_linear(ptr(x), ldx, ptr(codes), ptr(scale), ptr(zero), ptr(h), m, inter, k,
+                                              k // int(scale.shape[1]), DTYPES_16[x.dtype], _SCALE_DTYPES[scale.dtype],
+                                              activation, stream_ptr()), "fso_int4_gated_linear")
+    return h
+
+
+def int4_quantize(w, group: int, zero_point: bool, scale_dtype):
+    """16-bit w [N, K] -> (codes uint8 [N, K/2], scale [N, K/group], zero uint8 [N, K/group] or None)."""
+    n, k = int(w.shape[0]), int(w.shape[1])
+    with on_device(w.device):
+        codes = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
+        scale = torch.empty((n, k // group), dtype=scale_dtype, device=w.device)
+        zero = torch.empty((n, k // group), dtype=torch.uint8, device=w.device) if zero_point else None
+        check(lib().fso_int4_quantize(ptr(w), ptr(codes), ptr(scale), ptr(zero), n, k, int(group), DTYPES_16[w.dtype],
+                                      _SCALE_DTYPES[scale_dtype], stream_ptr()), "fso_int4_quantize")
+    return codes, scale, zero

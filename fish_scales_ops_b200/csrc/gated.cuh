@@ -1,0 +1,802 @@
+// The gated feed-forward projection in 16 bits, h = act(x G^T) * (x U^T), and its gradients, on CTA pairs:
+//
+//   forward    g = x G^T, u = x U^T            A = x, B = rows of G and U side by side; act and product in the epilogue
+//   dx         dg G + du U                     A = [dg | du], B = [G ; U], the two halves of the contraction in turn
+//   dG, dU     dg^T x, du^T x                  A = dg^T or du^T, B = x
+//
+// with dg = dh * u * act'(g), du = dh * act(g) (gated_slopes_kernel). All three are one kernel, a 256 x 256 tile for
+// each pair of CTAs (tcgen05.mma kind::f16, cta_group::2, fp32 accumulators in tensor memory), fed by TMA. The operand
+// whose contraction runs down its columns (G, U in dx; all operands of dG, dU) is staged as it lies in memory and
+// read by the tensor cores "M/N-major": nothing is transposed in memory.
+//
+// What bounds it: the tensor pipe for T from a few hundred on (an MMA of 256 x 256 x 16 takes 128 cycles), the weight
+// bytes below that.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "gemm_host.cuh"
+
+namespace fso {
+
+enum : int { G16_GATED = 0, G16_DX = 1, G16_DW = 2 };
+enum : int { FSO_ACT_SILU = 0, FSO_ACT_GELU = 1, FSO_ACT_GELU_TANH = 2 };
+
+struct Gated16Cfg {
+    static constexpr int kStages = 6;
+    static constexpr int kEpiWarps = 8;
+    static constexpr int kThreads = 128 + 32 * kEpiWarps;
+    static constexpr int kOpBytes = 128 * 128;          // one operand of one CTA and stage: 128 rows x 64 elements
+    static constexpr int kStageBytes = 2 * kOpBytes;
+    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 512;
+    static constexpr int kTmemCols = 512;               // two accumulators of 256 columns
+    static_assert(kSmemBytes <= 227 * 1024 && kSmemBytes > 116 * 1024, "one CTA per SM");
+};
+
+struct Gated16Params {
+    int rows;            // valid rows of the output (G16_DW: of one half)
+    int cols;            // valid columns of the output
+    int tiles_m;         // 256-row tiles (G16_DW: of both halves)
+    int tiles_half;      // G16_DW: 256-row tiles of one half
+    int tiles_n;
+    int group_m;         // raster: row tiles walked together before the columns advance
+    int kb_total;        // 64-wide blocks of the contraction
+    int kb_half;         // G16_DX: blocks of the first half
+    int splits;
+    int kb_per_split;
+    int act;
+    int vec;             // rows of `out` start on 16-byte boundaries
+    void* out;           // 16 bit [rows, ldo]
+    int64_t ldo;
+    int64_t out_half;    // G16_DW: elements from the first half's output to the second's
+    uint16_t* save_hi;   // G16_GATED: upper 16 of the 24 bits kept of g and u, [rows, 2 * half_cols], or nullptr
+    uint8_t* save_lo;    // G16_GATED: lower 8 bits
+    int64_t half_cols;   // columns from g to u in the saved arrays and in split sums
+    float* ws;           // splits > 1: fp32 sums [splits, rows, ws_cols] (G16_DW: [splits, 2, rows, ws_cols])
+    int64_t ws_cols;
+};
+
+// ------------------------------------------------------------------------------------------------ activations
+//
+// a = act(g) and s = act'(g), from act(g) = g P(g): P is the logistic function of g (silu), the normal distribution
+// function (gelu), or the logistic function of 2 z, z = sqrt(2/pi) (g + 0.044715 g^3), which is 0.5 (1 + tanh z).
+// The logistic function goes through the exponential and one division, so its relative error stays below 1e-5 in both
+// tails; 16-bit outputs cannot see it.
+__device__ __forceinline__ float logistic(float v) { return 1.f / (1.f + __expf(-v)); }
+
+constexpr float kGeluC = 0.79788456080286535588f;      // sqrt(2 / pi)
+constexpr float kGeluCubic = 0.044715f;
+
+__device__ __forceinline__ float gate_value(float g, int act)
+{
+    if (act == FSO_ACT_SILU) return g * logistic(g);
+    if (act == FSO_ACT_GELU) return g * normcdff(g);
+    return g * logistic(2.f * kGeluC * (g + kGeluCubic * g * g * g));
+}
+
+__device__ __forceinline__ void gate_value_slope(float g, int act, float& a, float& s)
+{
+    float p, dp;      // dp = g P'(g)
+    if (act == FSO_ACT_SILU) {
+        p = logistic(g);
+        dp = g * p * logistic(-g);
+    } else if (act == FSO_ACT_GELU) {
+        p = normcdff(g);
+        dp = g * 0.39894228040143267794f * __expf(-0.5f * g * g);
+    } else {
+        float const z2 = 2.f * kGeluC * (g + kGeluCubic * g * g * g);
+        p = logistic(z2);
+        dp = g * p * logistic(-z2) * 2.f * kGeluC * (1.f + 3.f * kGeluCubic * g * g);
+    }
+    a = g * p;
+    s = p + dp;
+}
+
+// ------------------------------------------------------------------------------------------------ 16-bit and 24-bit values
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi)
+{
+    if constexpr (kBf16) {
+        __nv_bfloat162 const v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t const*>(&v);
+    } else {
+        __half2 const v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t const*>(&v);
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ float2 unpack16(uint32_t w)
+{
+    if constexpr (kBf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    else return __half22float2(*reinterpret_cast<__half2 const*>(&w));
+}
+
+template <bool kBf16>
+__device__ __forceinline__ float load16(const void* p, int64_t i)
+{
+    if constexpr (kBf16) return __bfloat162float(static_cast<__nv_bfloat16 const*>(p)[i]);
+    else return __half2float(static_cast<__half const*>(p)[i]);
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void store16(void* p, int64_t i, float v)
+{
+    if constexpr (kBf16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// g and u are kept for the backward pass in 24 bits (the upper 24 of the fp32 value, rounded): in 16 bits their
+// rounding would be as large as the one that dg and du go through on the way to the tensor cores and would raise the
+// error of the gradients by a quarter; three bytes instead of four cost the pass less memory and traffic.
+// Only finite values are rounded up: an infinity or a NaN keeps its upper bits, and a NaN keeps its quiet bit there.
+__device__ __forceinline__ uint32_t to_24(float v)
+{
+    uint32_t const b = __float_as_uint(v);
+    return ((b & 0x7F800000u) == 0x7F800000u ? b : b + 0x80u) >> 8;
+}
+
+__device__ __forceinline__ float from_24(uint32_t hi, uint32_t lo) { return __uint_as_float((hi << 16) | (lo << 8)); }
+
+// 16 consecutive fp32 values of one row, the first `valid` of them inside the row, to 16 bits.
+template <bool kBf16>
+__device__ __forceinline__ void store_row16(void* out, int64_t at, float const (&v)[16], int valid, bool vec)
+{
+    if (vec) {      // rows start on 16-byte boundaries and `at` is a multiple of 16 inside the row
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            if (8 * q + 8 <= valid) {
+                uint4 const w = make_uint4(pack16<kBf16>(v[8 * q], v[8 * q + 1]), pack16<kBf16>(v[8 * q + 2], v[8 * q + 3]),
+                    pack16<kBf16>(v[8 * q + 4], v[8 * q + 5]), pack16<kBf16>(v[8 * q + 6], v[8 * q + 7]));
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at + 8 * q) = w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < valid) store16<kBf16>(out, at + j, v[j]);
+    }
+}
+
+// 16 consecutive g (or u) values of one row to the saved arrays, whose rows are padded to multiples of 16 columns.
+__device__ __forceinline__ void store_saved(uint16_t* hi, uint8_t* lo, int64_t at, float const (&v)[16])
+{
+    uint32_t h[8], l[4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        uint32_t const a = to_24(v[2 * j]), b = to_24(v[2 * j + 1]);
+        h[j] = (a >> 8) | ((b >> 8) << 16);
+        uint32_t const two = (a & 0xFFu) | ((b & 0xFFu) << 8);
+        if (j & 1) l[j >> 1] |= two << 16;
+        else l[j >> 1] = two;
+    }
+    uint4* const dh = reinterpret_cast<uint4*>(hi + at);
+    dh[0] = make_uint4(h[0], h[1], h[2], h[3]);
+    dh[1] = make_uint4(h[4], h[5], h[6], h[7]);
+    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+// ------------------------------------------------------------------------------------------------ tensor-core forms
+
+// Instruction descriptor of kind::f16 over a CTA pair: fp32 accumulator, both operands bf16 or both fp16, M = 256,
+// N = 256; `a_mn` / `b_mn`: the operand is stored with its M (N) dimension contiguous.
+__host__ __device__ constexpr uint32_t make_idesc_f16_pair(bool bf16, bool a_mn, bool b_mn)
+{
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u)
+        | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+}
+
+// Descriptor of an operand tile stored with its M (or N) dimension contiguous: blocks of 64 elements (128 bytes, the
+// 128-byte swizzle) x 64 contraction steps, 8 KB each, one block behind the other. Inside a block eight steps are
+// 1024 bytes. Advancing by 16 steps adds 2048 bytes.
+__device__ __forceinline__ uint64_t make_desc_mn_sw128(uint32_t saddr)
+{
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(8192 >> 4) << 16;           // between 64-element blocks
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;           // between groups of eight steps
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tc_mma_f16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+    uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------ the kernel
+//
+// The protocol is that of gemm_mxf8_pair_kernel (gemm2.cuh): both CTAs' producers load their own shared memory and
+// count bytes on the leader's barrier, the leader issues the MMAs of the pair, each CTA runs its own epilogue. Without
+// scale factors two accumulators of 256 columns fill tensor memory, so a tile's epilogue runs under the next tile's
+// MMAs. Forward: CTA 0 stages 128 rows of G, CTA 1 the same 128 rows of U, so a CTA's accumulator holds g in columns
+// 0..127 and u in columns 128..255 of its own 128 tokens.
+template <int MODE, bool kBf16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Gated16Cfg::kThreads, 1)
+gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constant__ CUtensorMap tm_a1,
+    const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1, const Gated16Params p)
+{
+    using C = Gated16Cfg;
+    constexpr int S = C::kStages;
+    constexpr bool kAmn = MODE == G16_DW, kBmn = MODE != G16_GATED;
+    extern __shared__ uint8_t smem_raw[];
+    uint32_t const raw = smem_u32(smem_raw);
+    uint32_t const base = (raw + 1023u) & ~1023u;
+    uint8_t* const gbase = smem_raw + (base - raw);
+    uint32_t const sA = base;
+    uint32_t const sB = sA + S * C::kOpBytes;
+    uint32_t const bars = sB + S * C::kOpBytes;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
+    auto tfull_bar = [&](int a) { return bars + 8u * (2 * S + a); };
+    auto tempty_bar = [&](int a) { return bars + 8u * (2 * S + 2 + a); };
+    uint32_t const misc_off = static_cast<uint32_t>(S) * C::kStageBytes + 8u * (2 * S + 4);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + misc_off);
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(gbase + misc_off + 4);
+
+    int const warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+    int const lane = threadIdx.x & 31;
+    uint32_t const rank = cluster_ctarank();
+    bool const leader = rank == 0;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), 2 * C::kEpiWarps);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+        prefetch_tensormap(&tm_a0);
+        prefetch_tensormap(&tm_b0);
+        prefetch_tensormap(&tm_b1);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(tmem_slot), C::kTmemCols);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    uint32_t const tmem_base = *tmem_slot;
+
+    int const pair = blockIdx.x >> 1;
+    int const num_pairs = gridDim.x >> 1;
+    int const tiles = p.tiles_m * p.tiles_n;
+    int const items = tiles * p.splits;
+
+    struct Item {
+        int tile_m, tile_n, split, kb0, kb1, half;
+    };
+    auto decode = [&](int t) {
+        Item c;
+        c.split = t / tiles;
+        int const r = t - c.split * tiles;
+        int const span = p.group_m * p.tiles_n;
+        int const g = r / span;
+        int const first = g * p.group_m;
+        int const gsz = min(p.group_m, p.tiles_m - first);
+        int const in_g = r - g * span;
+        c.tile_n = in_g / gsz;
+        c.tile_m = first + (in_g - c.tile_n * gsz);
+        c.half = 0;
+        if constexpr (MODE == G16_DW) {
+            c.half = c.tile_m >= p.tiles_half ? 1 : 0;
+            c.tile_m -= c.half * p.tiles_half;
+        }
+        c.kb0 = c.split * p.kb_per_split;
+        c.kb1 = min(p.kb_total, c.kb0 + p.kb_per_split);
+        return c;
+    };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------------------------ TMA producer (both CTAs)
+        if (elect_one()) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < items; t += num_pairs) {
+                Item const c = decode(t);
+                int const a0 = c.tile_m * 256 + static_cast<int>(rank) * 128;
+                int const b0 = MODE == G16_GATED ? c.tile_n * 128 : c.tile_n * 256 + static_cast<int>(rank) * 128;
+                for (int kb = c.kb0; kb < c.kb1; ++kb) {
+                    if (!wait_or_abort(empty_bar(stage), phase ^ 1u, abort_flag)) {
+                        record_abort(FSO_DEV_WAIT_PRODUCER, abort_flag);
+                        ok = false;
+                        break;
+                    }
+                    uint32_t const fb = map_to_cta(full_bar(stage), 0);
+                    if (leader) mbar_expect_tx(full_bar(stage), 2u * C::kStageBytes);
+                    uint32_t const da = sA + stage * C::kOpBytes, db = sB + stage * C::kOpBytes;
+                    if constexpr (MODE == G16_GATED) {
+                        tma_load_2d_pair(da, &tm_a0, fb, kb * 64, a0);
+                        tma_load_2d_pair(db, rank == 0 ? &tm_b0 : &tm_b1, fb, kb * 64, b0);
+                    } else if constexpr (MODE == G16_DX) {
+                        bool const second = kb >= p.kb_half;
+                        int const kc = (second ? kb - p.kb_half : kb) * 64;
+                        const CUtensorMap* const tb = second ? &tm_b1 : &tm_b0;
+                        tma_load_2d_pair(da, second ? &tm_a1 : &tm_a0, fb, kc, a0);
+                        tma_load_2d_pair(db, tb, fb, b0, kc);
+                        tma_load_2d_pair(db + 8192, tb, fb, b0 + 64, kc);
+                    } else {
+                        const CUtensorMap* const ta = c.half ? &tm_a1 : &tm_a0;
+                        tma_load_2d_pair(da, ta, fb, a0, kb * 64);
+                        tma_load_2d_pair(da + 8192, ta, fb, a0 + 64, kb * 64);
+                        tma_load_2d_pair(db, &tm_b0, fb, b0, kb * 64);
+                        tma_load_2d_pair(db + 8192, &tm_b0, fb, b0 + 64, kb * 64);
+                    }
+                    if (++stage == S) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------------------------ MMA issuer (leader only)
+        if (leader && elect_one()) {
+            int stage = 0;
+            uint32_t phase = 0;
+            int acc = 0;
+            uint32_t acc_phase = 0;
+            constexpr uint32_t idesc = make_idesc_f16_pair(kBf16, kAmn, kBmn);
+            bool ok = true;
+            for (int t = pair; ok && t < items; t += num_pairs) {
+                Item const c = decode(t);
+                if (!wait_or_abort(tempty_bar(acc), acc_phase ^ 1u, abort_flag)) {
+                    record_abort(FSO_DEV_WAIT_MMA_TMEM, abort_flag);
+                    break;
+                }
+                tc_fence_after();
+                uint32_t const d_tmem = tmem_base + static_cast<uint32_t>(acc * 256);
+                for (int kb = c.kb0; kb < c.kb1; ++kb) {
+                    if (!wait_or_abort(full_bar(stage), phase, abort_flag)) {
+                        record_abort(FSO_DEV_WAIT_MMA_FULL, abort_flag);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    uint32_t const sa = sA + stage * C::kOpBytes, sb = sB + stage * C::kOpBytes;
+                    uint64_t const adesc = kAmn ? make_desc_mn_sw128(sa) : make_desc_sw128(sa);
+                    uint64_t const bdesc = kBmn ? make_desc_mn_sw128(sb) : make_desc_sw128(sb);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)      // 16 elements of the contraction: 32 bytes of a row, or 16 rows
+                        tc_mma_f16_pair(d_tmem, adesc + (kAmn ? 128u : 2u) * k, bdesc + (kBmn ? 128u : 2u) * k, idesc,
+                            (kb > c.kb0 || k > 0) ? 1u : 0u);
+                    tc_commit_pair_both(empty_bar(stage));
+                    if (++stage == S) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                tc_commit_pair_both(tfull_bar(acc));
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------------------------------ epilogue (both CTAs)
+        int const quarter = warp & 3;
+        int const half = (warp - 4) >> 2;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int t = pair; t < items; t += num_pairs) {
+            Item const c = decode(t);
+            if (!wait_or_abort(tfull_bar(acc), acc_phase, abort_flag)) {
+                if (lane == 0) record_abort(FSO_DEV_WAIT_EPILOGUE, abort_flag);
+                break;
+            }
+            tc_fence_after();
+            uint32_t const t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * 256);
+            int const row = c.tile_m * 256 + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+            bool const live = row < p.rows;
+            if constexpr (MODE == G16_GATED) {
+#pragma unroll 1
+                for (int j = 0; j < 4; ++j) {
+                    __syncwarp();      // lanes past the last row skip the stores below
+                    int const in_tile = half * 64 + 16 * j;
+                    uint32_t rg[16], ru[16];
+                    tmem_ld_32x16(t_row + in_tile, rg);
+                    tmem_ld_32x16(t_row + 128 + in_tile, ru);
+                    tmem_ld_wait();
+                    int const col = c.tile_n * 128 + in_tile;
+                    if (!live || col >= p.cols) continue;
+                    float g[16], u[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        g[i] = __uint_as_float(rg[i]);
+                        u[i] = __uint_as_float(ru[i]);
+                    }
+                    if (p.ws != nullptr) {
+                        float* const w = p.ws + (static_cast<int64_t>(c.split) * p.rows + row) * p.ws_cols + col;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            reinterpret_cast<float4*>(w)[i] = make_float4(g[4 * i], g[4 * i + 1], g[4 * i + 2], g[4 * i + 3]);
+                            reinterpret_cast<float4*>(w + p.half_cols)[i] =
+                                make_float4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+                        }
+                        continue;
+                    }
+                    if (p.save_hi != nullptr) {
+                        int64_t const at = static_cast<int64_t>(row) * 2 * p.half_cols + col;
+                        store_saved(p.save_hi, p.save_lo, at, g);
+                        store_saved(p.save_hi, p.save_lo, at + p.half_cols, u);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) g[i] = gate_value(g[i], p.act) * u[i];
+                    store_row16<kBf16>(p.out, static_cast<int64_t>(row) * p.ldo + col, g, p.cols - col, p.vec != 0);
+                }
+            } else {
+#pragma unroll 1
+                for (int j = 0; j < 8; ++j) {
+                    __syncwarp();
+                    int const in_tile = half * 128 + 16 * j;
+                    uint32_t r[16];
+                    tmem_ld_32x16(t_row + in_tile, r);
+                    tmem_ld_wait();
+                    int const col = c.tile_n * 256 + in_tile;
+                    if (!live || col >= p.cols) continue;
+                    float v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+                    if (p.ws != nullptr) {
+                        int64_t const slab = MODE == G16_DW ? 2 * c.split + c.half : c.split;
+                        float* const w = p.ws + (slab * p.rows + row) * p.ws_cols + col;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            reinterpret_cast<float4*>(w)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        continue;
+                    }
+                    store_row16<kBf16>(p.out, c.half * p.out_half + static_cast<int64_t>(row) * p.ldo + col, v, p.cols - col,
+                        p.vec != 0);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_cta(tempty_bar(acc), 0));
+            if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1u;
+            }
+        }
+        __syncwarp();
+    }
+
+    // ---------------------------------------------------------------------------------------- teardown
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+        __syncthreads();
+    }
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, C::kTmemCols);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ split sums
+
+// out = the sum of the slices of the contraction, in their order, rounded once. Columns are multiples of 8.
+template <bool kBf16>
+__global__ void gated16_sum_kernel(float const* __restrict__ ws, int splits, int64_t slab, int64_t rows, int cols,
+    int64_t ws_cols, uint16_t* __restrict__ out, int64_t ldo)
+{
+    int const per_row = cols / 8;
+    int64_t const i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i >= rows * per_row) return;
+    int64_t const row = i / per_row;
+    int const col = static_cast<int>(i - row * per_row) * 8;
+    float v[8] = {};
+    for (int s = 0; s < splits; ++s) {
+        float4 const* const w = reinterpret_cast<float4 const*>(ws + s * slab + row * ws_cols + col);
+        float4 const a = w[0], b = w[1];
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    }
+    *reinterpret_cast<uint4*>(out + row * ldo + col) = make_uint4(pack16<kBf16>(v[0], v[1]), pack16<kBf16>(v[2], v[3]),
+        pack16<kBf16>(v[4], v[5]), pack16<kBf16>(v[6], v[7]));
+}
+
+// The epilogue of the forward pass for a split contraction: sums, saved values, act and product. 16 columns a thread.
+template <bool kBf16>
+__global__ void gated16_finish_kernel(float const* __restrict__ ws, int splits, int rows, int cols, int64_t half_cols,
+    int act, uint16_t* __restrict__ save_hi, uint8_t* __restrict__ save_lo, void* __restrict__ out, int vec)
+{
+    int const per_row = static_cast<int>(half_cols / 16);
+    int64_t const i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i >= static_cast<int64_t>(rows) * per_row) return;
+    int64_t const row = i / per_row;
+    int const col = static_cast<int>(i - row * per_row) * 16;
+    float g[16] = {}, u[16] = {};
+    for (int s = 0; s < splits; ++s) {
+        float const* const w = ws + (static_cast<int64_t>(s) * rows + row) * 2 * half_cols + col;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            g[j] += w[j];
+            u[j] += w[half_cols + j];
+        }
+    }
+    if (save_hi != nullptr) {
+        int64_t const at = row * 2 * half_cols + col;
+        store_saved(save_hi, save_lo, at, g);
+        store_saved(save_hi, save_lo, at + half_cols, u);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) g[j] = gate_value(g[j], act) * u[j];
+    store_row16<kBf16>(out, row * cols + col, g, cols - col, vec != 0);
+}
+
+// ------------------------------------------------------------------------------------------------ dg and du
+//
+// dg = dh * u * act'(g), du = dh * act(g) from the saved g and u, rounded to the 16 bits in which the tensor cores take
+// them (the one rounding of the backward pass before its products). Bound by memory: 2 + 2 * 3 bytes in and 4 out for
+// each element. Eight columns a thread.
+template <bool kBf16>
+__global__ void gated_slopes_kernel(const void* __restrict__ dh, int64_t ldh, int dh_vec, uint16_t const* __restrict__ save_hi,
+    uint8_t const* __restrict__ save_lo, int rows, int cols, int64_t half_cols, int act, uint16_t* __restrict__ out)
+{
+    int const per_row = static_cast<int>(half_cols / 8);
+    int64_t const i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i >= static_cast<int64_t>(rows) * per_row) return;
+    int64_t const row = i / per_row;
+    int const col = static_cast<int>(i - row * per_row) * 8;
+    if (col >= cols) return;
+    float d[8];
+    if (dh_vec) {
+        uint4 const w = *reinterpret_cast<uint4 const*>(static_cast<uint16_t const*>(dh) + row * ldh + col);
+        uint32_t const q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 const f = unpack16<kBf16>(q[j]);
+            d[2 * j] = f.x;
+            d[2 * j + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = col + j < cols ? load16<kBf16>(dh, row * ldh + col + j) : 0.f;
+    }
+    int64_t const at = row * 2 * half_cols + col;
+    uint4 const gh = *reinterpret_cast<uint4 const*>(save_hi + at), uh = *reinterpret_cast<uint4 const*>(save_hi + at + half_cols);
+    uint2 const gl = *reinterpret_cast<uint2 const*>(save_lo + at), ul = *reinterpret_cast<uint2 const*>(save_lo + at + half_cols);
+    uint32_t const ghw[4] = {gh.x, gh.y, gh.z, gh.w}, uhw[4] = {uh.x, uh.y, uh.z, uh.w};
+    uint32_t const glw[2] = {gl.x, gl.y}, ulw[2] = {ul.x, ul.y};
+    float dg[8], du[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float const g = from_24((ghw[j / 2] >> (16 * (j & 1))) & 0xFFFFu, (glw[j / 4] >> (8 * (j & 3))) & 0xFFu);
+        float const u = from_24((uhw[j / 2] >> (16 * (j & 1))) & 0xFFFFu, (ulw[j / 4] >> (8 * (j & 3))) & 0xFFu);
+        float a, s;
+        gate_value_slope(g, act, a, s);
+        dg[j] = d[j] * u * s;
+        du[j] = d[j] * a;
+    }
+    *reinterpret_cast<uint4*>(out + at) = make_uint4(pack16<kBf16>(dg[0], dg[1]), pack16<kBf16>(dg[2], dg[3]),
+        pack16<kBf16>(dg[4], dg[5]), pack16<kBf16>(dg[6], dg[7]));
+    *reinterpret_cast<uint4*>(out + at + half_cols) = make_uint4(pack16<kBf16>(du[0], du[1]), pack16<kBf16>(du[2], du[3]),
+        pack16<kBf16>(du[4], du[5]), pack16<kBf16>(du[6], du[7]));
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+
+// Tensor map of a 16-bit matrix [rows, cols] with `ld` elements between rows, read in boxes of 64 columns x box_rows
+// with the 128-byte swizzle; what a box holds outside the matrix reads as zero.
+inline int make_map16(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows)
+{
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) {
+        set_error("cuTensorMapEncodeTiled is not available from this driver");
+        return FSO_ERR_UNSUPPORTED;
+    }
+    cuuint64_t const dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    cuuint64_t const strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+    cuuint32_t const box[2] = {64u, static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t const estr[2] = {1u, 1u};
+    CUresult const r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed with CUresult %d (16-bit matrix of %lld x %lld, %lld between rows)",
+            static_cast<int>(r), static_cast<long long>(rows), static_cast<long long>(cols), static_cast<long long>(ld));
+        return FSO_ERR_INTERNAL;
+    }
+    return 0;
+}
+
+inline int64_t gated_half_cols(int64_t inter) { return (inter + 15) / 16 * 16; }
+
+// Tiles and slices of one of the three products. Pure host arithmetic.
+struct Gated16Plan {
+    int tiles_m, tiles_half, tiles_n, kb, kb_half, splits, kb_per_split;
+    int64_t ws_bytes;
+};
+
+inline Gated16Plan plan_gated16(int mode, int64_t t, int64_t k, int64_t inter, int sms)
+{
+    Gated16Plan p{};
+    auto tiles = [](int64_t n, int64_t w) { return static_cast<int>((n + w - 1) / w); };
+    int64_t rows = t, ws_cols = k;
+    if (mode == G16_GATED) {
+        p.tiles_m = tiles(t, 256);
+        p.tiles_n = tiles(inter, 128);
+        p.kb = tiles(k, 64);
+        ws_cols = 2 * gated_half_cols(inter);
+    } else if (mode == G16_DX) {
+        p.tiles_m = tiles(t, 256);
+        p.tiles_n = tiles(k, 256);
+        p.kb_half = tiles(inter, 64);
+        p.kb = 2 * p.kb_half;
+        ws_cols = (k + 15) / 16 * 16;
+    } else {
+        p.tiles_half = tiles(inter, 256);
+        p.tiles_m = 2 * p.tiles_half;
+        p.tiles_n = tiles(k, 256);
+        p.kb = tiles(t, 64);
+        rows = 2 * inter;
+        ws_cols = (k + 15) / 16 * 16;
+    }
+    // slices of the contraction where the tiles would leave half of the SM pairs without work
+    pick_splits(static_cast<int64_t>(p.tiles_m) * p.tiles_n, p.kb, sms / 2, 8, 16, &p.splits, &p.kb_per_split);
+    p.ws_bytes = p.splits > 1 ? p.splits * rows * ws_cols * 4 : 0;
+    return p;
+}
+
+template <int MODE, bool kBf16>
+inline int launch_gated16(CUtensorMap const (&m)[4], Gated16Params const& p, int sms, cudaStream_t stream)
+{
+    static std::atomic<uint64_t> done{0};
+    auto kernel = gated16_pair_kernel<MODE, kBf16>;
+    int const rc = ensure_smem_attr(kernel, Gated16Cfg::kSmemBytes, done);
+    if (rc != 0) return rc;
+    int64_t const items = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
+    int const pairs = static_cast<int>(std::min<int64_t>(items, std::max(1, sms / 2)));
+    kernel<<<2 * pairs, Gated16Cfg::kThreads, Gated16Cfg::kSmemBytes, stream>>>(m[0], m[1], m[2], m[3], p);
+    return launch_status("gated16_pair_kernel");
+}
+
+inline void fill_gated16(Gated16Params& p, Gated16Plan const& pl)
+{
+    p.tiles_m = pl.tiles_m;
+    p.tiles_half = pl.tiles_half;
+    p.tiles_n = pl.tiles_n;
+    p.group_m = std::min(pl.tiles_m, 8);
+    p.kb_total = pl.kb;
+    p.kb_half = pl.kb_half;
+    p.splits = pl.splits;
+    p.kb_per_split = pl.kb_per_split;
+}
+
+inline unsigned blocks_for(int64_t threads, int per_block) { return static_cast<unsigned>((threads + per_block - 1) / per_block); }
+
+template <bool kBf16>
+inline int gated_forward(const void* x, int64_t ldx, const void* gate_up, void* h, void* save_hi, void* save_lo, int64_t t,
+    int64_t k, int64_t inter, int act, void* ws, cudaStream_t stream)
+{
+    int const sms = sm_count();
+    Gated16Plan const pl = plan_gated16(G16_GATED, t, k, inter, sms);
+    CUtensorMap m[4];
+    uint16_t const* const w = static_cast<uint16_t const*>(gate_up);
+    int rc = make_map16(&m[0], x, t, k, ldx, 128);
+    if (rc == 0) rc = make_map16(&m[2], w, inter, k, k, 128);
+    if (rc == 0) rc = make_map16(&m[3], w + inter * k, inter, k, k, 128);
+    if (rc != 0) return rc;
+    m[1] = m[0];
+    Gated16Params p{};
+    fill_gated16(p, pl);
+    p.rows = static_cast<int>(t);
+    p.cols = static_cast<int>(inter);
+    p.act = act;
+    p.vec = inter % 8 == 0 && aligned16(h);
+    p.out = h;
+    p.ldo = inter;
+    p.save_hi = static_cast<uint16_t*>(save_hi);
+    p.save_lo = static_cast<uint8_t*>(save_lo);
+    p.half_cols = gated_half_cols(inter);
+    p.ws = pl.splits > 1 ? static_cast<float*>(ws) : nullptr;
+    p.ws_cols = 2 * p.half_cols;
+    rc = launch_gated16<G16_GATED, kBf16>(m, p, sms, stream);
+    if (rc != 0 || pl.splits == 1) return rc;
+    gated16_finish_kernel<kBf16><<<blocks_for(t * (p.half_cols / 16), 128), 128, 0, stream>>>(p.ws, pl.splits, p.rows, p.cols,
+        p.half_cols, act, p.save_hi, p.save_lo, h, p.vec);
+    return launch_status("gated16_finish_kernel");
+}
+
+// Workspace of the backward pass: dg and du (16 bit [T, 2 * half_cols]), then the slices of whichever product has them.
+inline int64_t gated_backward_ws_bytes(int64_t t, int64_t k, int64_t inter, int sms)
+{
+    int64_t const slopes = (t * 2 * gated_half_cols(inter) * 2 + 255) / 256 * 256;
+    return slopes + std::max(plan_gated16(G16_DX, t, k, inter, sms).ws_bytes, plan_gated16(G16_DW, t, k, inter, sms).ws_bytes);
+}
+
+template <bool kBf16>
+inline int gated_backward(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* gate_up, const void* save_hi,
+    const void* save_lo, void* dx, void* dgate_up, int64_t t, int64_t k, int64_t inter, int act, void* ws, cudaStream_t stream)
+{
+    int const sms = sm_count();
+    int64_t const hc = gated_half_cols(inter);
+    uint16_t* const slopes = static_cast<uint16_t*>(ws);
+    float* const sums = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + (t * 2 * hc * 2 + 255) / 256 * 256);
+    int const dh_vec = inter % 8 == 0 && ldh % 8 == 0 && aligned16(dh);
+    gated_slopes_kernel<kBf16><<<blocks_for(t * (hc / 8), 256), 256, 0, stream>>>(dh, ldh, dh_vec,
+        static_cast<uint16_t const*>(save_hi), static_cast<uint8_t const*>(save_lo), static_cast<int>(t),
+        static_cast<int>(inter), hc, act, slopes);
+    int rc = launch_status("gated_slopes_kernel");
+    if (rc != 0) return rc;
+    uint16_t const* const w = static_cast<uint16_t const*>(gate_up);
+    if (dx != nullptr) {
+        Gated16Plan const pl = plan_gated16(G16_DX, t, k, inter, sms);
+        CUtensorMap m[4];
+        rc = make_map16(&m[0], slopes, t, inter, 2 * hc, 128);
+        if (rc == 0) rc = make_map16(&m[1], slopes + hc, t, inter, 2 * hc, 128);
+        if (rc == 0) rc = make_map16(&m[2], w, inter, k, k, 64);
+        if (rc == 0) rc = make_map16(&m[3], w + inter * k, inter, k, k, 64);
+        if (rc != 0) return rc;
+        Gated16Params p{};
+        fill_gated16(p, pl);
+        p.rows = static_cast<int>(t);
+        p.cols = static_cast<int>(k);
+        p.vec = 1;
+        p.out = dx;
+        p.ldo = k;
+        p.ws = pl.splits > 1 ? sums : nullptr;
+        p.ws_cols = (k + 15) / 16 * 16;
+        rc = launch_gated16<G16_DX, kBf16>(m, p, sms, stream);
+        if (rc != 0) return rc;
+        if (pl.splits > 1) {
+            gated16_sum_kernel<kBf16><<<blocks_for(t * (k / 8), 256), 256, 0, stream>>>(sums, pl.splits, t * p.ws_cols, t,
+                p.cols, p.ws_cols, static_cast<uint16_t*>(dx), k);
+            rc = launch_status("gated16_sum_kernel");
+            if (rc != 0) return rc;
+        }
+    }
+    if (dgate_up != nullptr) {
+        Gated16Plan const pl = plan_gated16(G16_DW, t, k, inter, sms);
+        CUtensorMap m[4];
+        rc = make_map16(&m[0], slopes, t, inter, 2 * hc, 64);
+        if (rc == 0) rc = make_map16(&m[1], slopes + hc, t, inter, 2 * hc, 64);
+        if (rc == 0) rc = make_map16(&m[2], x, t, k, ldx, 64);
+        if (rc != 0) return rc;
+        m[3] = m[2];
+        Gated16Params p{};
+        fill_gated16(p, pl);
+        p.rows = static_cast<int>(inter);
+        p.cols = static_cast<int>(k);
+        p.vec = 1;
+        p.out = dgate_up;
+        p.ldo = k;
+        p.out_half = inter * k;
+        p.ws = pl.splits > 1 ? sums : nullptr;
+        p.ws_cols = (k + 15) / 16 * 16;
+        rc = launch_gated16<G16_DW, kBf16>(m, p, sms, stream);
+        if (rc != 0) return rc;
+        if (pl.splits > 1) {
+            gated16_sum_kernel<kBf16><<<blocks_for(2 * inter * (k / 8), 256), 256, 0, stream>>>(sums, pl.splits,
+                2 * inter * p.ws_cols, 2 * inter, p.cols, p.ws_cols, static_cast<uint16_t*>(dgate_up), k);
+            rc = launch_status("gated16_sum_kernel");
+            if (rc != 0) return rc;
+        }
+    }
+    return 0;
+}
+
+}  // namespace fso

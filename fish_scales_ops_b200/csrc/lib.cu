@@ -41,6 +41,8 @@ int sm_count()
 #include "moe.cuh"
 #include "exchange.cuh"
 #include "router.cuh"
+#include "gated.cuh"
+#include "int4.cuh"
 
 using namespace fso;
 
@@ -671,6 +673,165 @@ int fso_moe_gather_rows(const void* rx_q, const void* rx_w, const int32_t* slot_
         static_cast<const uint4*>(rx_q), static_cast<const uint32_t*>(rx_w), slot_of_flat, rows_in,
         static_cast<int>(topk), static_cast<int>(h / 128), static_cast<uint4*>(hq), static_cast<uint32_t*>(sh));
     return launch_status("gather_rows_q_kernel");
+}
+
+// Sizes of the gated projection. Offsets into its tensors are 64 bits wide; the tensor maps take 32-bit coordinates.
+static int check_gated_shape(const char* op, int64_t t, int64_t k, int64_t inter, int64_t dtype, int64_t activation)
+{
+    FSO_REQUIRE(t >= 0 && k > 0 && inter > 0, "%s: T >= 0, K > 0 and INTER > 0 required", op);
+    FSO_REQUIRE(k % 8 == 0, "%s: K = %lld must be a multiple of 8", op, static_cast<long long>(k));
+    FSO_REQUIRE(t <= (1ll << 24) && k <= (1ll << 24) && inter <= (1ll << 24), "%s: dimension beyond 2^24", op);
+    FSO_REQUIRE(dtype == 0 || dtype == 1, "%s: dtype must be 0 (bf16) or 1 (fp16)", op);
+    FSO_REQUIRE(activation >= 0 && activation <= 2, "%s: activation must be 0 (silu), 1 (gelu) or 2 (gelu_tanh)", op);
+    return 0;
+}
+
+int fso_gated_linear_saved_cols(int64_t inter, int64_t* cols)
+{
+    FSO_REQUIRE(cols != nullptr && inter > 0, "fso_gated_linear_saved_cols: INTER > 0 and a place for the answer required");
+    *cols = 2 * gated_half_cols(inter);
+    return 0;
+}
+
+int fso_gated_linear_ws_bytes(int64_t t, int64_t k, int64_t inter, int64_t* bytes)
+{
+    FSO_REQUIRE(bytes != nullptr, "fso_gated_linear_ws_bytes: bytes is NULL");
+    int const rc = check_gated_shape("fso_gated_linear_ws_bytes", t, k, inter, 0, 0);
+    if (rc != 0) return rc;
+    *bytes = t == 0 ? 0 : plan_gated16(G16_GATED, t, k, inter, sm_count()).ws_bytes;
+    return 0;
+}
+
+int fso_gated_linear(const void* x, int64_t ldx, const void* gate_up, void* h, void* save_hi, void* save_lo, int64_t t,
+    int64_t k, int64_t inter, int64_t dtype, int64_t activation, void* ws, int64_t ws_bytes, void* stream)
+{
+    int const rc = check_gated_shape("fso_gated_linear", t, k, inter, dtype, activation);
+    if (rc != 0) return rc;
+    if (t == 0) return 0;
+    FSO_REQUIRE(x && gate_up && h, "fso_gated_linear: NULL pointer");
+    FSO_REQUIRE((save_hi == nullptr) == (save_lo == nullptr), "fso_gated_linear: save_hi and save_lo go together");
+    FSO_REQUIRE(ldx >= k && ldx % 8 == 0, "fso_gated_linear: ldx = %lld must be a multiple of 8 and at least K",
+        static_cast<long long>(ldx));
+    FSO_REQUIRE(aligned16(x) && aligned16(gate_up) && aligned16(save_hi) && aligned16(save_lo) && aligned16(ws),
+        "fso_gated_linear: x, gate_up, the saved arrays and the workspace must be 16-byte aligned");
+    int64_t const need = plan_gated16(G16_GATED, t, k, inter, sm_count()).ws_bytes;
+    FSO_REQUIRE(need == 0 || (ws != nullptr && ws_bytes >= need), "fso_gated_linear: workspace of %lld bytes required, got %lld",
+        static_cast<long long>(need), static_cast<long long>(ws == nullptr ? 0 : ws_bytes));
+    return dtype == 0 ? gated_forward<true>(x, ldx, gate_up, h, save_hi, save_lo, t, k, inter, static_cast<int>(activation), ws, as_stream(stream))
+                      : gated_forward<false>(x, ldx, gate_up, h, save_hi, save_lo, t, k, inter, static_cast<int>(activation), ws, as_stream(stream));
+}
+
+int fso_gated_linear_backward_ws_bytes(int64_t t, int64_t k, int64_t inter, int64_t* bytes)
+{
+    FSO_REQUIRE(bytes != nullptr, "fso_gated_linear_backward_ws_bytes: bytes is NULL");
+    int const rc = check_gated_shape("fso_gated_linear_backward_ws_bytes", t, k, inter, 0, 0);
+    if (rc != 0) return rc;
+    *bytes = t == 0 ? 0 : gated_backward_ws_bytes(t, k, inter, sm_count());
+    return 0;
+}
+
+int fso_gated_linear_backward(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* gate_up, const void* save_hi,
+    const void* save_lo, void* dx, void* dgate_up, int64_t t, int64_t k, int64_t inter, int64_t dtype, int64_t activation,
+    void* ws, int64_t ws_bytes, void* stream)
+{
+    int const rc = check_gated_shape("fso_gated_linear_backward", t, k, inter, dtype, activation);
+    if (rc != 0) return rc;
+    FSO_REQUIRE(t > 0, "fso_gated_linear_backward: T > 0 required (without rows dx is empty and dgate_up zero)");
+    FSO_REQUIRE(dh && x && gate_up && save_hi && save_lo && ws, "fso_gated_linear_backward: NULL pointer");
+    FSO_REQUIRE(ldx >= k && ldx % 8 == 0 && ldh >= inter,
+        "fso_gated_linear_backward: ldx = %lld must be a multiple of 8 and at least K, ldh = %lld at least INTER",
+        static_cast<long long>(ldx), static_cast<long long>(ldh));
+    FSO_REQUIRE(aligned16(x) && aligned16(gate_up) && aligned16(save_hi) && aligned16(save_lo) && aligned16(dx)
+            && aligned16(dgate_up) && aligned16(ws) && (reinterpret_cast<uintptr_t>(dh) & 1u) == 0,
+        "fso_gated_linear_backward: every operand but dh must be 16-byte aligned");
+    int64_t const need = gated_backward_ws_bytes(t, k, inter, sm_count());
+    FSO_REQUIRE(ws_bytes >= need, "fso_gated_linear_backward: workspace of %lld bytes required, got %lld",
+        static_cast<long long>(need), static_cast<long long>(ws_bytes));
+    return dtype == 0 ? gated_backward<true>(dh, ldh, x, ldx, gate_up, save_hi, save_lo, dx, dgate_up, t, k, inter,
+                            static_cast<int>(activation), ws, as_stream(stream))
+                      : gated_backward<false>(dh, ldh, x, ldx, gate_up, save_hi, save_lo, dx, dgate_up, t, k, inter,
+                            static_cast<int>(activation), ws, as_stream(stream));
+}
+
+static int check_int4(const char* op, int64_t m, int64_t rows, int64_t k, int64_t group, int64_t dtype, int64_t scale_dtype,
+    const void* x, int64_t ldx, const void* codes, const void* scale, const void* out)
+{
+    FSO_REQUIRE(m >= 0 && rows > 0 && k > 0, "%s: M >= 0, rows > 0 and K > 0 required", op);
+    FSO_REQUIRE(group >= 32 && (group & (group - 1)) == 0 && k % group == 0,
+        "%s: the group size %lld must be a power of two of at least 32 that divides K = %lld", op, static_cast<long long>(group),
+        static_cast<long long>(k));
+    FSO_REQUIRE(m <= 65535 * 8 && rows <= (1ll << 24) && k <= (1ll << 24), "%s: dimension too large", op);
+    FSO_REQUIRE((dtype == 0 || dtype == 1) && scale_dtype >= 0 && scale_dtype <= 2,
+        "%s: dtype must be 0 (bf16) or 1 (fp16), scale_dtype 0, 1 or 2 (fp32)", op);
+    if (m == 0) return 0;
+    FSO_REQUIRE(x && codes && scale && out, "%s: NULL pointer", op);
+    FSO_REQUIRE(ldx >= k && ldx % 8 == 0, "%s: ldx = %lld must be a multiple of 8 and at least K", op, static_cast<long long>(ldx));
+    FSO_REQUIRE(aligned16(x) && aligned16(codes), "%s: x and codes must be 16-byte aligned", op);
+    return 0;
+}
+
+int fso_int4_quantize(const void* w, void* codes, void* scale, void* zero, int64_t n, int64_t k, int64_t group, int64_t dtype,
+    int64_t scale_dtype, void* stream)
+{
+    FSO_REQUIRE(n > 0 && k > 0 && n <= (1ll << 24) && k <= (1ll << 24), "fso_int4_quantize: N and K must be in [1, 2^24]");
+    FSO_REQUIRE((group == 32 || group == 64 || group == 128 || group == 256) && k % group == 0,
+        "fso_int4_quantize: the group size must be 32, 64, 128 or 256 and divide K");
+    FSO_REQUIRE((dtype == 0 || dtype == 1) && scale_dtype >= 0 && scale_dtype <= 2,
+        "fso_int4_quantize: dtype must be 0 (bf16) or 1 (fp16), scale_dtype 0, 1 or 2 (fp32)");
+    FSO_REQUIRE(w && codes && scale, "fso_int4_quantize: NULL pointer");
+    FSO_REQUIRE(aligned16(w) && (reinterpret_cast<uintptr_t>(codes) & 3u) == 0 && (reinterpret_cast<uintptr_t>(scale) & 3u) == 0,
+        "fso_int4_quantize: w must be 16-byte aligned, codes and scale 4-byte aligned");
+    int64_t const vectors = n * (k / 8);
+    FSO_REQUIRE(vectors <= (1ll << 38), "fso_int4_quantize: N * K is too large for one launch");
+    auto kernel = dtype == 0 ? int4_quantize_kernel<true> : int4_quantize_kernel<false>;
+    kernel<<<blocks_for(vectors, 256), 256, 0, as_stream(stream)>>>(static_cast<uint4 const*>(w), static_cast<uint32_t*>(codes),
+        scale, static_cast<int>(scale_dtype), static_cast<uint8_t*>(zero), vectors, static_cast<int>(group / 8));
+    return launch_status("int4_quantize_kernel");
+}
+
+int fso_int4_linear(const void* x, int64_t ldx, const void* codes, const void* scale, const void* zero, const void* bias,
+    void* y, int64_t m, int64_t n, int64_t k, int64_t group, int64_t dtype, int64_t scale_dtype, void* stream)
+{
+    int const rc = check_int4("fso_int4_linear", m, n, k, group, dtype, scale_dtype, x, ldx, codes, scale, y);
+    if (rc != 0 || m == 0) return rc;
+    Int4Params p{};
+    p.x = x;
+    p.ldx = ldx;
+    p.codes = static_cast<uint8_t const*>(codes);
+    p.scale = scale;
+    p.scale_type = static_cast<int>(scale_dtype);
+    p.zero = static_cast<uint8_t const*>(zero);
+    p.bias = bias;
+    p.out = y;
+    p.m = static_cast<int>(m);
+    p.k = static_cast<int>(k);
+    p.group = static_cast<int>(group);
+    p.out_cols = static_cast<int>(n);
+    return launch_int4(p, dtype == 0, false, as_stream(stream));
+}
+
+int fso_int4_gated_linear(const void* x, int64_t ldx, const void* codes, const void* scale, const void* zero, void* h,
+    int64_t m, int64_t inter, int64_t k, int64_t group, int64_t dtype, int64_t scale_dtype, int64_t activation, void* stream)
+{
+    FSO_REQUIRE(inter > 0 && inter <= (1ll << 23), "fso_int4_gated_linear: INTER must be in [1, 2^23]");
+    FSO_REQUIRE(activation >= 0 && activation <= 2,
+        "fso_int4_gated_linear: activation must be 0 (silu), 1 (gelu) or 2 (gelu_tanh)");
+    int const rc = check_int4("fso_int4_gated_linear", m, 2 * inter, k, group, dtype, scale_dtype, x, ldx, codes, scale, h);
+    if (rc != 0 || m == 0) return rc;
+    Int4Params p{};
+    p.x = x;
+    p.ldx = ldx;
+    p.codes = static_cast<uint8_t const*>(codes);
+    p.scale = scale;
+    p.scale_type = static_cast<int>(scale_dtype);
+    p.zero = static_cast<uint8_t const*>(zero);
+    p.out = h;
+    p.m = static_cast<int>(m);
+    p.k = static_cast<int>(k);
+    p.group = static_cast<int>(group);
+    p.out_cols = static_cast<int>(inter);
+    p.act = static_cast<int>(activation);
+    return launch_int4(p, dtype == 0, true, as_stream(stream));
 }
 
 }  // extern "C"

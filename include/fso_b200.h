@@ -262,6 +262,49 @@ int fso_moe_combine_scatter(const void* dn, const int32_t* slot_of_flat, const f
                             int64_t topk, int64_t h, const int64_t* recv_off, const int64_t* back_base,
                             const uint64_t* peer_back, int64_t world, void* stream);
 
+/* ---- Gated feed-forward projection in 16 bits, with its gradients --------------------------------------------------
+ *
+ * h[t, i] = act(x[t] . G[i]) * (x[t] . U[i]), G and U the first and the last INTER rows of gate_up [2 * INTER, K].
+ * dtype: 0 = bf16, 1 = fp16 (x, gate_up, h and the gradients alike). activation: 0 = silu, 1 = gelu (erf),
+ * 2 = gelu with tanh. K % 8 == 0; INTER and T are free. x [T, ldx]: ldx elements between rows, ldx % 8 == 0. h, dx and
+ * dgate_up are contiguous. Sums are fp32; h is rounded once. No counterpart in the reference, whose gate_up projection is
+ * MXFP8 and forward only (python/fish_scales_ops/gemm/mxfp8.py:216-236).
+ *
+ * save_hi (uint16 [T, saved_cols]) and save_lo (uint8 [T, saved_cols]), both NULL or both given, receive g = x G^T and
+ * u = x U^T in 24 bits for the backward pass; fso_gated_linear_saved_cols answers saved_cols. The workspace holds the
+ * slices of a contraction that was split; its size comes from the _ws_bytes query for the same sizes, 0 where none is
+ * needed. */
+int fso_gated_linear_saved_cols(int64_t inter, int64_t* cols);
+int fso_gated_linear_ws_bytes(int64_t t, int64_t k, int64_t inter, int64_t* bytes);
+int fso_gated_linear(const void* x, int64_t ldx, const void* gate_up, void* h, void* save_hi, void* save_lo, int64_t t,
+                     int64_t k, int64_t inter, int64_t dtype, int64_t activation, void* ws, int64_t ws_bytes, void* stream);
+
+/* Gradients of the above for dh [T, ldh]: with dg = dh * u * act'(g) and du = dh * act(g), rounded to dtype,
+ * dx = dg G + du U and dgate_up = [dg^T x ; du^T x]. dx or dgate_up may be NULL where it is not wanted. */
+int fso_gated_linear_backward_ws_bytes(int64_t t, int64_t k, int64_t inter, int64_t* bytes);
+int fso_gated_linear_backward(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* gate_up,
+                              const void* save_hi, const void* save_lo, void* dx, void* dgate_up, int64_t t, int64_t k,
+                              int64_t inter, int64_t dtype, int64_t activation, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- Linear layers over 4-bit weights with group scales ------------------------------------------------------------
+ *
+ * W[n, k] = scale[n, k / group] * (code[n, k] - zero[n, k / group]); codes two in a byte, even k in the lower four bits,
+ * rows of K / 2 bytes; scale bf16 (0), fp16 (1) or fp32 (2) [N, K / group]; zero uint8 of the same shape, or NULL for 8.
+ * group is a power of two of at least 32 that divides K. x 16 bit [M, ldx] (dtype 0 = bf16, 1 = fp16), ldx % 8 == 0; codes
+ * and x 16-byte aligned. y[m] = x[m] W^T (+ bias), h[m] = act(x[m] G^T) * (x[m] U^T) with G, U the first and the last
+ * INTER rows of W; both contiguous. The whole number code - zero enters its product exactly, sums and scales are
+ * fp32, the result is rounded once. Built for the few rows of a decode step. No counterpart in the reference, which
+ * serves 8-bit weights (python/fish_scales_ops/dense/__init__.py:121-140). */
+/* 16-bit w [N, K] -> codes, scale and (zero not NULL) zero points by rounding each group to its nearest steps: amax / 7
+ * around 8, or (hi - lo) / 15 with zero inside the range; group 32, 64, 128 or 256. */
+int fso_int4_quantize(const void* w, void* codes, void* scale, void* zero, int64_t n, int64_t k, int64_t group, int64_t dtype,
+                      int64_t scale_dtype, void* stream);
+int fso_int4_linear(const void* x, int64_t ldx, const void* codes, const void* scale, const void* zero, const void* bias,
+                    void* y, int64_t m, int64_t n, int64_t k, int64_t group, int64_t dtype, int64_t scale_dtype, void* stream);
+int fso_int4_gated_linear(const void* x, int64_t ldx, const void* codes, const void* scale, const void* zero, void* h,
+                          int64_t m, int64_t inter, int64_t k, int64_t group, int64_t dtype, int64_t scale_dtype,
+                          int64_t activation, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
