@@ -16,15 +16,20 @@ namespace fso {
 struct Int4Params {
     const void* x;         // 16 bit [m, ldx]
     int64_t ldx;
-    const uint8_t* codes;  // [rows, k / 2]
-    const void* scale;     // [rows, k / group]
+    const void* scale;     // [rows, groups]
     int scale_type;        // 0 bf16, 1 fp16, 2 fp32
-    const uint8_t* zero;   // [rows, k / group], or nullptr: 8
-    const void* bias;      // [out], 16 bit like x, or nullptr
+    const uint8_t* zero;   // [rows, groups], or nullptr: 8
+    const void* bias;      // [out_cols], 16 bit like x, or nullptr
     void* out;             // 16 bit [m, out_cols]
-    int m, k, group;
+    int m, k;
+    int group_shift;       // log2 of the group size
+    int groups;            // groups of a row
     int out_cols;          // rows of the weight, or half of them when gated
+    int gated;
     int act;
+    int steps;             // 512-wide steps of the contraction
+    int steps_per_slice;
+    int splits;            // slices of the contraction = CTAs of a cluster
 };
 
 __device__ __forceinline__ float int4_scale(Int4Params const& p, int64_t i)
@@ -34,62 +39,316 @@ __device__ __forceinline__ float int4_scale(Int4Params const& p, int64_t i)
     return static_cast<float const*>(p.scale)[i];
 }
 
-// One warp for each output column and eight rows of x; a lane takes eight consecutive k of every 256.
-template <bool kBf16, bool kGated>
-__global__ void int4_rows_kernel(Int4Params const p)
+// Eight codes of a word to the eight 16-bit numbers code - zero, exactly: a code in the low bits of the mantissa of 128
+// (bf16) or 1024 (fp16) is 128 + code, and taking away 128 + zero is exact. Register i gets the codes i and i + 4, which
+// lie 16 bits apart. `zero2` is that minuend twice.
+template <bool kBf16>
+__device__ __forceinline__ void int4_unpack(uint32_t w, uint32_t zero2, uint32_t (&r)[4])
 {
+    constexpr uint32_t kOne = kBf16 ? 0x43004300u : 0x64006400u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t v;
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w >> (4 * i)), "n"(0x000F000F), "n"(kOne));      // (a & b) | c
+        if constexpr (kBf16) {
+            __nv_bfloat162 const d = __hsub2(*reinterpret_cast<__nv_bfloat162 const*>(&v), *reinterpret_cast<__nv_bfloat162 const*>(&zero2));
+            r[i] = *reinterpret_cast<uint32_t const*>(&d);
+        } else {
+            __half2 const d = __hsub2(*reinterpret_cast<__half2 const*>(&v), *reinterpret_cast<__half2 const*>(&zero2));
+            r[i] = *reinterpret_cast<uint32_t const*>(&d);
+        }
+    }
+}
+
+// c += A (16 rows x 16 of the contraction) * B (16 x 8 columns), fp32 sums, one warp.
+template <bool kBf16>
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+    uint32_t b1)
+{
+    if constexpr (kBf16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t saddr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(saddr) : "memory");
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
+struct Int4Cfg {
+    static constexpr int kRows = 64;             // weight rows of a CTA (gated: 32 of each half)
+    static constexpr int kStep = 512;            // of the contraction in a stage, 128 for each of the four warps
+    static constexpr int kWarps = 4;
+    static constexpr int kThreads = 32 * kWarps + 32;
+    static constexpr int kStages = 6;
+    static constexpr int kStageBytes = kRows * kStep / 2;
+    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+    static constexpr int kRedStride = kRows + 4; // floats between the rows of x in the partial sums: lanes hit 32 banks
+    static_assert(2 * (kSmemBytes + 1024) <= 227 * 1024, "two CTAs per SM");
+};
+
+// The few rows of x of a decode step (at most 8 * NT in a CTA) against 64 rows of the weight.
+//
+// Bound by the weight bytes, so they are streamed by TMA, six stages of 16 KB deep and two CTAs to an SM, and everything
+// else is sized to stay below the time of a stage. A warp turns its codes into tensor-core fragments in registers
+// (mma.sync: the 16-row side is the weight, eight rows of x are one tile; decode never fills a tcgen05 tile, and the
+// codes would have to go through shared memory once more to get there). ldmatrix hands a lane the word that holds
+// the eight codes k = 8 t .. 8 t + 7 of its weight row; any order of the contraction will do as long as x follows it, so the
+// pairs (i, i + 4) that the masks give are met by permuted registers of x, which come straight from global memory. The
+// sums of a group are scaled in fp32 as they leave the tensor cores. The four warps split a stage along the contraction,
+// which leaves each its own part of x, and add up at the end; the CTAs of a cluster split it further where rows are
+// few, and each adds up a part of the outputs over distributed shared memory, in a fixed order.
+//
+// GC: 32-wide chunks of a group inside the 128 of a warp (4 for groups of 128 and more).
+template <bool kBf16, int NT, int GC>
+__global__ void __launch_bounds__(Int4Cfg::kThreads, 2)
+int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ CUtensorMap tm_hi, const Int4Params p)
+{
+    using C = Int4Cfg;
+    constexpr int S = C::kStages;
+    constexpr int G = 4 / GC;      // groups of a warp and stage
+    extern __shared__ uint8_t smem_raw[];
+    uint32_t const raw = smem_u32(smem_raw);
+    uint32_t const base = (raw + 1023u) & ~1023u;
+    uint8_t* const gbase = smem_raw + (base - raw);
+    uint32_t const bars = base + S * C::kStageBytes;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(gbase + S * C::kStageBytes + 16 * S);
+
+    int const warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
     int const lane = threadIdx.x & 31;
-    int64_t const col = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5);
-    if (col >= p.out_cols) return;
-    int const t0 = blockIdx.y * 8;
-    int const live = min(8, p.m - t0);
-    int const groups = p.k / p.group;
-    float sums[kGated ? 2 : 1][8];
+    int const tile = blockIdx.x / p.splits;
+    int const rank = blockIdx.x - tile * p.splits;
+    int const step0 = rank * p.steps_per_slice;
+    int const step1 = min(p.steps, step0 + p.steps_per_slice);
+    int const t0 = blockIdx.y * (8 * NT);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), C::kWarps);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    __syncthreads();
+    griddep_launch_dependents();
+
+    float tot[4][NT][4] = {};
+    if (warp == C::kWarps) {
+        // -------------------------------------------------------------------------------- weight stream (immutable bytes:
+        // it starts under the preceding kernel)
+        if (elect_one()) {
+            int const row_lo = tile * (p.gated ? 32 : 64);
+            int const row_hi = p.gated ? row_lo : row_lo + 32;
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int st = step0; st < step1; ++st) {
+                if (!wait_or_abort(empty_bar(stage), phase ^ 1u, abort_flag)) {
+                    record_abort(FSO_DEV_WAIT_PRODUCER, abort_flag);
+                    break;
+                }
+                uint32_t const fb = full_bar(stage), dst = base + stage * C::kStageBytes;
+                mbar_expect_tx(fb, C::kStageBytes);
 #pragma unroll
-    for (int half = 0; half < (kGated ? 2 : 1); ++half) {
-        int64_t const row = col + static_cast<int64_t>(half) * p.out_cols;
-        float acc[8] = {};
-        for (int k0 = lane * 8; k0 < p.k; k0 += 256) {
-            uint32_t const w = *reinterpret_cast<uint32_t const*>(p.codes + row * (p.k / 2) + k0 / 2);
-            int64_t const at = row * groups + k0 / p.group;
-            float const s = int4_scale(p, at);
-            int const z = p.zero != nullptr ? p.zero[at] : 8;
-            float q[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = static_cast<float>(static_cast<int>((w >> (4 * j)) & 15u) - z);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                if (t < live) {
-                    uint4 const v = *reinterpret_cast<uint4 const*>(
-                        static_cast<uint16_t const*>(p.x) + static_cast<int64_t>(t0 + t) * p.ldx + k0);
-                    uint32_t const words[4] = {v.x, v.y, v.z, v.w};
-                    float part = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float2 const f = unpack16<kBf16>(words[j]);
-                        part = fmaf(q[2 * j], f.x, part);
-                        part = fmaf(q[2 * j + 1], f.y, part);
-                    }
-                    acc[t] = fmaf(s, part, acc[t]);
+                for (int b = 0; b < 2; ++b) {
+                    tma_load_2d(dst + b * 8192, &tm_lo, fb, st * (C::kStep / 2) + b * 128, row_lo);
+                    tma_load_2d(dst + b * 8192 + 4096, &tm_hi, fb, st * (C::kStep / 2) + b * 128, row_hi);
+                }
+                if (++stage == S) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
         }
+        __syncwarp();
+    } else {
+        int const g = lane >> 2, t = lane & 3;
+        // lane l looks after the scales of rows l and l + 32 of the tile; rows past the last one borrow its scales
+        int64_t srow[2];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
+        for (int h = 0; h < 2; ++h) {
+            int const r = p.gated ? min(tile * 32 + lane, p.out_cols - 1) + h * p.out_cols
+                                  : min(tile * 64 + h * 32 + lane, p.out_cols - 1);
+            srow[h] = static_cast<int64_t>(r) * p.groups;
+        }
+        float sc[2][G];
+        uint32_t zz[2][G];
+        auto load_scales = [&](int k0) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
-            sums[half][t] = acc[t];
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    int const gi = min((k0 + 32 * GC * j) >> p.group_shift, p.groups - 1);
+                    sc[h][j] = int4_scale(p, srow[h] + gi);
+                    uint32_t const z = p.zero != nullptr ? p.zero[srow[h] + gi] : 8u;
+                    zz[h][j] = ((kBf16 ? 0x4300u : 0x6400u) + z) * 0x10001u;
+                }
+        };
+        // x in the order of the B fragments: lane (g, t) takes row g and the elements 8 t .. 8 t + 7 of each chunk
+        uint16_t const* xrow[NT];
+        bool live[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            live[n] = t0 + 8 * n + g < p.m;
+            xrow[n] = static_cast<uint16_t const*>(p.x) + static_cast<int64_t>(live[n] ? t0 + 8 * n + g : 0) * p.ldx + 8 * t;
+        }
+        uint4 xv[4][NT];
+        auto load_x = [&](int k0) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    xv[c][n] = live[n] && k0 + 32 * c < p.k ? *reinterpret_cast<uint4 const*>(xrow[n] + k0 + 32 * c)
+                                                            : make_uint4(0, 0, 0, 0);
+        };
+        // ldmatrix: lanes 8 i .. 8 i + 7 give the rows of matrix i: rows 0-7 and 8-15 of a chunk, then of the next chunk
+        uint32_t const mrow = ((lane >> 3) & 1) * 8 + (lane & 7);
+        uint32_t const mchunk = (warp & 1) * 4 + (lane >> 4);
+        uint32_t const moff = (warp >> 1) * 8192 + mrow * 128;
+        uint32_t const moff0 = moff + ((mchunk ^ (lane & 7)) << 4), moff2 = moff + (((mchunk + 2) ^ (lane & 7)) << 4);
+
+        load_scales(step0 * C::kStep + warp * 128);
+        griddep_wait();
+        load_x(step0 * C::kStep + warp * 128);
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int st = step0; st < step1; ++st) {
+            int const k_next = (st + 1) * C::kStep + warp * 128;
+            uint32_t bx[4][NT][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    uint4 const v = xv[c][n];
+                    bx[c][n][0] = __byte_perm(v.x, v.z, 0x5410);      // elements 0 and 4
+                    bx[c][n][1] = __byte_perm(v.x, v.z, 0x7632);      // 1 and 5
+                    bx[c][n][2] = __byte_perm(v.y, v.w, 0x5410);      // 2 and 6
+                    bx[c][n][3] = __byte_perm(v.y, v.w, 0x7632);      // 3 and 7
+                }
+            float s_cur[2][G];
+            uint32_t z_cur[2][G];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    s_cur[h][j] = sc[h][j];
+                    z_cur[h][j] = zz[h][j];
+                }
+            if (st + 1 < step1) {
+                load_x(k_next);
+                load_scales(k_next);
+            }
+            if (!wait_or_abort(full_bar(stage), phase, abort_flag)) {
+                if (lane == 0) record_abort(FSO_DEV_WAIT_MMA_FULL, abort_flag);
+                break;
+            }
+            __syncwarp();
+            uint32_t const sbase = base + stage * C::kStageBytes;
+#pragma unroll
+            for (int rt = 0; rt < 4; ++rt) {
+                uint32_t w[2][4];
+                ldmatrix_x4(sbase + moff0 + rt * 2048, w[0]);
+                ldmatrix_x4(sbase + moff2 + rt * 2048, w[1]);
+                float acc[NT][4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    constexpr uint32_t kAll = 0xffffffffu;
+                    int const j = c / GC, src = (rt & 1) * 16 + g;
+                    uint32_t const z0 = __shfl_sync(kAll, z_cur[rt >> 1][j], src), z8 = __shfl_sync(kAll, z_cur[rt >> 1][j], src + 8);
+                    if (c % GC == 0) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+                    }
+                    uint32_t a[4], b[4];      // codes of row g and of row g + 8
+                    int4_unpack<kBf16>(w[c >> 1][2 * (c & 1)], z0, a);
+                    int4_unpack<kBf16>(w[c >> 1][2 * (c & 1) + 1], z8, b);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma_16x8x16<kBf16>(acc[n], a[0], b[0], a[1], b[1], bx[c][n][0], bx[c][n][1]);
+                        mma_16x8x16<kBf16>(acc[n], a[2], b[2], a[3], b[3], bx[c][n][2], bx[c][n][3]);
+                    }
+                    if (c % GC == GC - 1) {
+                        float const s0 = __shfl_sync(kAll, s_cur[rt >> 1][j], src), s8 = __shfl_sync(kAll, s_cur[rt >> 1][j], src + 8);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            tot[rt][n][0] = fmaf(s0, acc[n][0], tot[rt][n][0]);
+                            tot[rt][n][1] = fmaf(s0, acc[n][1], tot[rt][n][1]);
+                            tot[rt][n][2] = fmaf(s8, acc[n][2], tot[rt][n][2]);
+                            tot[rt][n][3] = fmaf(s8, acc[n][3], tot[rt][n][3]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty_bar(stage));
+            if (++stage == S) {
+                stage = 0;
+                phase ^= 1u;
+            }
         }
     }
+
+    // ---------------------------------------------------------------------------------------- sums of the warps and slices
+    __syncthreads();      // every stage has been read: the ring becomes [warp][row of x][weight row]
+    bool const failed = *abort_flag != 0;
+    if (failed) {
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);      // copies in flight land before the memory is given up
+        __syncthreads();
+    }
+    float* const red = reinterpret_cast<float*>(gbase);
+    constexpr int kWarpFloats = 8 * NT * C::kRedStride;
+    static_assert(C::kWarps * kWarpFloats * 4 <= S * C::kStageBytes, "partial sums fit the ring");
+    if (warp < C::kWarps) {
+        int const g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-        if (lane == t && t < live) {
-            float v = sums[0][t];
-            if constexpr (kGated) v = gate_value(v, p.act) * sums[1][t];
+        for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    red[warp * kWarpFloats + (8 * n + 2 * t + (q & 1)) * C::kRedStride + rt * 16 + g + 8 * (q >> 1)] = tot[rt][n][q];
+    }
+    cluster_sync_all();
+    if (warp < C::kWarps && !failed) {
+        int const cols = p.gated ? 32 : 64;
+        int const rows = min(8 * NT, p.m - t0);
+        uint32_t const red_addr = smem_u32(red);
+        auto sum_of = [&](int row, int col) {
+            float v = 0.f;
+            for (int r = 0; r < p.splits; ++r) {
+                uint32_t const peer = map_to_cta(red_addr + 4u * (row * C::kRedStride + col), r);
+#pragma unroll
+                for (int w = 0; w < C::kWarps; ++w) v += ld_cluster_f32(peer + 4u * (w * kWarpFloats));
+            }
+            return v;
+        };
+        for (int i = rank * 128 + static_cast<int>(threadIdx.x); i < rows * cols; i += 128 * p.splits) {
+            int const row = i / cols, in_tile = i - row * cols;
+            int const col = tile * cols + in_tile;
+            if (col >= p.out_cols) continue;
+            float v = sum_of(row, in_tile);
+            if (p.gated) v = gate_value(v, p.act) * sum_of(row, in_tile + 32);
             else if (p.bias != nullptr) v += load16<kBf16>(p.bias, col);
-            store16<kBf16>(p.out, static_cast<int64_t>(t0 + t) * p.out_cols + col, v);
+            store16<kBf16>(p.out, static_cast<int64_t>(t0 + row) * p.out_cols + col, v);
         }
     }
+    __syncwarp();
+    cluster_sync_all();      // no CTA leaves while another may still read its sums
 }
 
 // ------------------------------------------------------------------------------------------------ 16-bit weight -> 4 bits
@@ -148,14 +407,75 @@ __global__ void int4_quantize_kernel(const uint4* __restrict__ w, uint32_t* __re
     }
 }
 
-inline int launch_int4(Int4Params const& p, bool bf16, bool gated, cudaStream_t stream)
+// Tensor map of the codes [rows, k / 2] in boxes of 128 bytes x box_rows with the 128-byte swizzle.
+inline int make_codes_map(CUtensorMap* map, const uint8_t* codes, int64_t rows, int64_t k, int box_rows)
 {
-    dim3 const grid(static_cast<unsigned>((p.out_cols + 3) / 4), static_cast<unsigned>((p.m + 7) / 8));
-    if (bf16 && gated) int4_rows_kernel<true, true><<<grid, 128, 0, stream>>>(p);
-    else if (bf16) int4_rows_kernel<true, false><<<grid, 128, 0, stream>>>(p);
-    else if (gated) int4_rows_kernel<false, true><<<grid, 128, 0, stream>>>(p);
-    else int4_rows_kernel<false, false><<<grid, 128, 0, stream>>>(p);
+    return make_operand_map(map, codes, rows, k / 2, box_rows);
+}
+
+// Slices of the contraction for `tiles` CTAs' worth of rows: as many as it takes for all SMs to have CTAs (two fit), at
+// most eight (the portable cluster size), and no empty one.
+inline void int4_slices(int64_t tiles, int sms, Int4Params& p)
+{
+    int s = 1;
+    while (s < 8 && tiles * s * 2 <= 3 * sms && s * 2 <= p.steps) ++s;
+    p.steps_per_slice = (p.steps + s - 1) / s;
+    p.splits = (p.steps + p.steps_per_slice - 1) / p.steps_per_slice;
+}
+
+template <bool kBf16, int NT, int GC>
+inline int launch_int4_inst(CUtensorMap const& lo, CUtensorMap const& hi, Int4Params const& p, dim3 grid, cudaStream_t stream)
+{
+    static std::atomic<uint64_t> done{0};
+    auto kernel = int4_rows_kernel<kBf16, NT, GC>;
+    int const rc = ensure_smem_attr(kernel, Int4Cfg::kSmemBytes, done);
+    if (rc != 0) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(Int4Cfg::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = Int4Cfg::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(p.splits);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1 + pdl_attribute(&attr[1]);
+    FSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, lo, hi, p));
     return launch_status("int4_rows_kernel");
+}
+
+template <bool kBf16, int NT>
+inline int launch_int4_group(int group, CUtensorMap const& lo, CUtensorMap const& hi, Int4Params const& p, dim3 grid,
+    cudaStream_t stream)
+{
+    return group == 32 ? launch_int4_inst<kBf16, NT, 1>(lo, hi, p, grid, stream)
+        : group == 64 ? launch_int4_inst<kBf16, NT, 2>(lo, hi, p, grid, stream)
+                      : launch_int4_inst<kBf16, NT, 4>(lo, hi, p, grid, stream);
+}
+
+// p: everything but the fields that are derived here.
+inline int launch_int4(Int4Params p, const uint8_t* codes, int64_t group, bool bf16, cudaStream_t stream)
+{
+    p.group_shift = 0;
+    while ((1ll << p.group_shift) < group) ++p.group_shift;
+    p.groups = p.k >> p.group_shift;
+    p.steps = (p.k + Int4Cfg::kStep - 1) / Int4Cfg::kStep;
+    int const per_tile = p.gated ? 32 : 64;
+    int const tiles = (p.out_cols + per_tile - 1) / per_tile;
+    int4_slices(tiles, sm_count(), p);
+    CUtensorMap lo, hi;
+    int rc = make_codes_map(&lo, codes, p.out_cols, p.k, 32);
+    if (rc != 0) return rc;
+    hi = lo;
+    if (p.gated) rc = make_codes_map(&hi, codes + static_cast<int64_t>(p.out_cols) * (p.k / 2), p.out_cols, p.k, 32);
+    if (rc != 0) return rc;
+    int const nt = p.m <= 8 ? 1 : 2;
+    dim3 const grid(static_cast<unsigned>(tiles * p.splits), static_cast<unsigned>((p.m + 8 * nt - 1) / (8 * nt)));
+    int const gi = static_cast<int>(std::min<int64_t>(group, 128));
+    if (bf16) return nt == 1 ? launch_int4_group<true, 1>(gi, lo, hi, p, grid, stream) : launch_int4_group<true, 2>(gi, lo, hi, p, grid, stream);
+    return nt == 1 ? launch_int4_group<false, 1>(gi, lo, hi, p, grid, stream) : launch_int4_group<false, 2>(gi, lo, hi, p, grid, stream);
 }
 
 }  // namespace fso

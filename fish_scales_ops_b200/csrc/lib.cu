@@ -797,7 +797,6 @@ int fso_int4_linear(const void* x, int64_t ldx, const void* codes, const void* s
     Int4Params p{};
     p.x = x;
     p.ldx = ldx;
-    p.codes = static_cast<uint8_t const*>(codes);
     p.scale = scale;
     p.scale_type = static_cast<int>(scale_dtype);
     p.zero = static_cast<uint8_t const*>(zero);
@@ -805,9 +804,8 @@ int fso_int4_linear(const void* x, int64_t ldx, const void* codes, const void* s
     p.out = y;
     p.m = static_cast<int>(m);
     p.k = static_cast<int>(k);
-    p.group = static_cast<int>(group);
     p.out_cols = static_cast<int>(n);
-    return launch_int4(p, dtype == 0, false, as_stream(stream));
+    return launch_int4(p, static_cast<uint8_t const*>(codes), group, dtype == 0, as_stream(stream));
 }
 
 int fso_int4_gated_linear(const void* x, int64_t ldx, const void* codes, const void* scale, const void* zero, void* h,
@@ -821,17 +819,16 @@ int fso_int4_gated_linear(const void* x, int64_t ldx, const void* codes, const v
     Int4Params p{};
     p.x = x;
     p.ldx = ldx;
-    p.codes = static_cast<uint8_t const*>(codes);
     p.scale = scale;
     p.scale_type = static_cast<int>(scale_dtype);
     p.zero = static_cast<uint8_t const*>(zero);
     p.out = h;
     p.m = static_cast<int>(m);
     p.k = static_cast<int>(k);
-    p.group = static_cast<int>(group);
     p.out_cols = static_cast<int>(inter);
+    p.gated = 1;
     p.act = static_cast<int>(activation);
-    return launch_int4(p, dtype == 0, true, as_stream(stream));
+    return launch_int4(p, static_cast<uint8_t const*>(codes), group, dtype == 0, as_stream(stream));
 }
 
 }  // extern "C"

@@ -93,6 +93,13 @@ def _need_arch(op: str) -> None:
         raise NotImplementedError(f"{op}: this build serves sm_100-family devices")
 
 
+def _complete(handle: Int4Weight) -> Int4Weight:
+    """One empty plain launch behind whatever wrote the handle's tensors: a call on it starts to load the weight before
+    its predecessor on the stream has finished, which is only safe when that predecessor did not write it."""
+    _ops.stream_fence(handle.codes.device)
+    return handle
+
+
 def _aligned(t):
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -164,7 +171,7 @@ def prepare_weight(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torc
     _check_weight(ctx, codes, scale, zero)
     _need_arch(ctx)
     k = 2 * int(codes.shape[1])
-    return Int4Weight(device_arch(), k, int(codes.shape[0]), k // int(scale.shape[1]), codes, scale, zero)
+    return _complete(Int4Weight(device_arch(), k, int(codes.shape[0]), k // int(scale.shape[1]), codes, scale, zero))
 
 
 def quantize_weight(w: torch.Tensor, *, group_size: int = 128, zero_point: bool = False,
@@ -187,7 +194,7 @@ def quantize_weight(w: torch.Tensor, *, group_size: int = 128, zero_point: bool 
         raise ValueError(f"{ctx}: scale_dtype must be bf16, fp16 or fp32, got {scale_dtype}")
     _need_arch(ctx)
     codes, scale, zero = _ops.int4_quantize(_aligned(w.detach()), group_size, bool(zero_point), scale_dtype)
-    return Int4Weight(device_arch(), int(w.shape[1]), int(w.shape[0]), int(group_size), codes, scale, zero)
+    return _complete(Int4Weight(device_arch(), int(w.shape[1]), int(w.shape[0]), int(group_size), codes, scale, zero))
 
 
 def _flatten(x, weight, ctx: str):
