@@ -133,6 +133,17 @@ def on_device(device):
     return torch.cuda.device(idx)
 
 
+def call_on(x: torch.Tensor, call, *args):
+    """``call(*args, stream)`` with the current stream of ``x``'s device, which is made the current device for the call when
+    it is not already. Pointers go as plain integers (None for NULL). For calls that a decode step makes: every
+    microsecond of host time counts there."""
+    dev = x.get_device()
+    if dev == torch._C._cuda_getDevice():
+        return call(*args, torch._C._cuda_getCurrentRawStream(dev))
+    with torch.cuda.device(dev):
+        return call(*args, torch._C._cuda_getCurrentRawStream(dev))
+
+
 def stream_ptr():
     """The current stream of the current device as a raw handle (no Stream object is built: this sits on the path of
     every call)."""

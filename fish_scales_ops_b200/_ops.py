@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import MoePlan, check, lib, on_device, ptr, stream_ptr
+from ._lib import MoePlan, call_on, check, lib, on_device, ptr, stream_ptr
 
 FP8 = torch.float8_e4m3fn
 
@@ -395,27 +395,31 @@ def gated_linear_backward(dh, x, gate_up, hi, lo, activation: int, need_x: bool,
 
 def int4_linear(x, codes, scale, zero, bias):
     """x [M, K] and a 4-bit weight of N rows -> y [M, N]."""
-    m, k, n = int(x.shape[0]), int(x.shape[1]), int(codes.shape[0])
-    with on_device(x.device):
-        y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-        if m > 0:
-            x, ldx = rows_in_place(x)
-            check(lib().fso_int4_linear(ptr(x), ldx, ptr(codes), ptr(scale), ptr(zero), ptr(bias), ptr(y), m, n, k,
-                                        k // int(scale.shape[1]), DTYPES_16[x.dtype], _SCALE_DTYPES[scale.dtype],
-                                        stream_ptr()), "fso_int4_linear")
+    m, k = x.shape
+    n = codes.shape[0]
+    y = x.new_empty((m, n))
+    if m > 0:
+        x, ldx = rows_in_place(x)
+        rc = call_on(x, lib().fso_int4_linear, x.data_ptr(), ldx, codes.data_ptr(), scale.data_ptr(),
+                     None if zero is None else zero.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), m, n,
+                     k, k // scale.shape[1], DTYPES_16[x.dtype], _SCALE_DTYPES[scale.dtype])
+        if rc != 0:
+            check(rc, "fso_int4_linear")
     return y
 
 
 def int4_gated_linear(x, codes, scale, zero, activation: int):
     """x [M, K] and a 4-bit gate_up of 2I rows -> h [M, I]."""
-    m, k, inter = int(x.shape[0]), int(x.shape[1]), int(codes.shape[0]) // 2
-    with on_device(x.device):
-        h = torch.empty((m, inter), dtype=x.dtype, device=x.device)
-        if m > 0:
-            x, ldx = rows_in_place(x)
-            check(lib().fso_int4_gated_linear(ptr(x), ldx, ptr(codes), ptr(scale), ptr(zero), ptr(h), m, inter, k,
-                                              k // int(scale.shape[1]), DTYPES_16[x.dtype], _SCALE_DTYPES[scale.dtype],
-                                              activation, stream_ptr()), "fso_int4_gated_linear")
+    m, k = x.shape
+    inter = codes.shape[0] // 2
+    h = x.new_empty((m, inter))
+    if m > 0:
+        x, ldx = rows_in_place(x)
+        rc = call_on(x, lib().fso_int4_gated_linear, x.data_ptr(), ldx, codes.data_ptr(), scale.data_ptr(),
+                     None if zero is None else zero.data_ptr(), h.data_ptr(), m, inter, k, k // scale.shape[1],
+                     DTYPES_16[x.dtype], _SCALE_DTYPES[scale.dtype], activation)
+        if rc != 0:
+            check(rc, "fso_int4_gated_linear")
     return h
 
 

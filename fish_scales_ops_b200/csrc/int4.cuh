@@ -66,11 +66,11 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t
     uint32_t b1)
 {
     if constexpr (kBf16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -88,13 +88,16 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
     return v;
 }
 
+template <int NT>
 struct Int4Cfg {
     static constexpr int kRows = 64;             // weight rows of a CTA (gated: 32 of each half)
-    static constexpr int kStep = 512;            // of the contraction in a stage, 128 for each of the four warps
-    static constexpr int kWarps = 4;
+    static constexpr int kStep = 512;            // of the contraction in a stage, 128 for a warp
+    static constexpr int kWarps = 8;             // four along the contraction, two along the rows
     static constexpr int kThreads = 32 * kWarps + 32;
-    static constexpr int kStages = 6;
-    static constexpr int kStageBytes = kRows * kStep / 2;
+    static constexpr int kStages = NT == 1 ? 4 : 3;
+    static constexpr int kWeightBytes = kRows * kStep / 2;
+    static constexpr int kXBytes = 8 * NT * kStep * 2;
+    static constexpr int kStageBytes = kWeightBytes + kXBytes;
     static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
     static constexpr int kRedStride = kRows + 4; // floats between the rows of x in the partial sums: lanes hit 32 banks
     static_assert(2 * (kSmemBytes + 1024) <= 227 * 1024, "two CTAs per SM");
@@ -102,22 +105,23 @@ struct Int4Cfg {
 
 // The few rows of x of a decode step (at most 8 * NT in a CTA) against 64 rows of the weight.
 //
-// Bound by the weight bytes, so they are streamed by TMA, six stages of 16 KB deep and two CTAs to an SM, and everything
-// else is sized to stay below the time of a stage. A warp turns its codes into tensor-core fragments in registers
+// Bound by the weight bytes, so they are streamed by TMA, 48 to 64 KB deep and two CTAs to an SM, and everything else is
+// sized to stay below the time of a stage. A warp turns its codes into tensor-core fragments in registers
 // (mma.sync: the 16-row side is the weight, eight rows of x are one tile; decode never fills a tcgen05 tile, and the
 // codes would have to go through shared memory once more to get there). ldmatrix hands a lane the word that holds
 // the eight codes k = 8 t .. 8 t + 7 of its weight row; any order of the contraction will do as long as x follows it, so the
-// pairs (i, i + 4) that the masks give are met by permuted registers of x, which come straight from global memory. The
-// sums of a group are scaled in fp32 as they leave the tensor cores. The four warps split a stage along the contraction,
-// which leaves each its own part of x, and add up at the end; the CTAs of a cluster split it further where rows are
-// few, and each adds up a part of the outputs over distributed shared memory, in a fixed order.
+// pairs (i, i + 4) that the masks give are met by permuted registers of x. The sums of a group are scaled in fp32 as
+// they leave the tensor cores. Four pairs of warps split a stage along the contraction and add up at the end; the CTAs
+// of a cluster split it further where rows are few, and each adds up a part of the outputs over distributed shared
+// memory, in a fixed order.
 //
 // GC: 32-wide chunks of a group inside the 128 of a warp (4 for groups of 128 and more).
 template <bool kBf16, int NT, int GC>
-__global__ void __launch_bounds__(Int4Cfg::kThreads, 2)
-int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ CUtensorMap tm_hi, const Int4Params p)
+__global__ void __launch_bounds__(Int4Cfg<NT>::kThreads, 2)
+int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ CUtensorMap tm_hi,
+    const __grid_constant__ CUtensorMap tm_x, const Int4Params p)
 {
-    using C = Int4Cfg;
+    using C = Int4Cfg<NT>;
     constexpr int S = C::kStages;
     constexpr int G = 4 / GC;      // groups of a warp and stage
     extern __shared__ uint8_t smem_raw[];
@@ -148,20 +152,15 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
     __syncthreads();
     griddep_launch_dependents();
 
-    float tot[4][NT][4] = {};
+    int const kq = warp & 3, rh = (warp >> 2) & 1;      // this warp's quarter of a step and half of the rows
+    float tot[2][NT][4] = {};
     if (warp == C::kWarps) {
         // -------------------------------------------------------------------------------- weight stream (immutable bytes:
         // it starts under the preceding kernel)
         if (elect_one()) {
             int const row_lo = tile * (p.gated ? 32 : 64);
             int const row_hi = p.gated ? row_lo : row_lo + 32;
-            int stage = 0;
-            uint32_t phase = 0;
-            for (int st = step0; st < step1; ++st) {
-                if (!wait_or_abort(empty_bar(stage), phase ^ 1u, abort_flag)) {
-                    record_abort(FSO_DEV_WAIT_PRODUCER, abort_flag);
-                    break;
-                }
+            auto load_weight = [&](int stage, int st) {
                 uint32_t const fb = full_bar(stage), dst = base + stage * C::kStageBytes;
                 mbar_expect_tx(fb, C::kStageBytes);
 #pragma unroll
@@ -169,6 +168,27 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
                     tma_load_2d(dst + b * 8192, &tm_lo, fb, st * (C::kStep / 2) + b * 128, row_lo);
                     tma_load_2d(dst + b * 8192 + 4096, &tm_hi, fb, st * (C::kStep / 2) + b * 128, row_hi);
                 }
+            };
+            auto load_x = [&](int stage, int st) {
+                uint32_t const dst = base + stage * C::kStageBytes + C::kWeightBytes;
+#pragma unroll
+                for (int b = 0; b < 8; ++b)
+                    tma_load_2d(dst + b * (1024 * NT), &tm_x, full_bar(stage), st * C::kStep + b * 64, t0);
+            };
+            // the first stages are free; x may still be in the making
+            int const npre = min(S, step1 - step0);
+            for (int i = 0; i < npre; ++i) load_weight(i, step0 + i);
+            griddep_wait();
+            for (int i = 0; i < npre; ++i) load_x(i, step0 + i);
+            int stage = npre == S ? 0 : npre;
+            uint32_t phase = npre == S ? 1u : 0u;
+            for (int st = step0 + npre; st < step1; ++st) {
+                if (!wait_or_abort(empty_bar(stage), phase ^ 1u, abort_flag)) {
+                    record_abort(FSO_DEV_WAIT_PRODUCER, abort_flag);
+                    break;
+                }
+                load_weight(stage, st);
+                load_x(stage, st);
                 if (++stage == S) {
                     stage = 0;
                     phase ^= 1u;
@@ -178,119 +198,101 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
         __syncwarp();
     } else {
         int const g = lane >> 2, t = lane & 3;
-        // lane l looks after the scales of rows l and l + 32 of the tile; rows past the last one borrow its scales
-        int64_t srow[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            int const r = p.gated ? min(tile * 32 + lane, p.out_cols - 1) + h * p.out_cols
-                                  : min(tile * 64 + h * 32 + lane, p.out_cols - 1);
-            srow[h] = static_cast<int64_t>(r) * p.groups;
-        }
-        float sc[2][G];
-        uint32_t zz[2][G];
+        // lane l looks after the scales of row l of the warp's 32; rows past the last one borrow its scales
+        int const srow = p.gated ? min(tile * 32 + lane, p.out_cols - 1) + rh * p.out_cols
+                                 : min(tile * 64 + rh * 32 + lane, p.out_cols - 1);
+        int64_t const sbase0 = static_cast<int64_t>(srow) * p.groups;
+        float sc[G];
+        uint32_t zz[G];
         auto load_scales = [&](int k0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    int const gi = min((k0 + 32 * GC * j) >> p.group_shift, p.groups - 1);
-                    sc[h][j] = int4_scale(p, srow[h] + gi);
-                    uint32_t const z = p.zero != nullptr ? p.zero[srow[h] + gi] : 8u;
-                    zz[h][j] = ((kBf16 ? 0x4300u : 0x6400u) + z) * 0x10001u;
-                }
-        };
-        // x in the order of the B fragments: lane (g, t) takes row g and the elements 8 t .. 8 t + 7 of each chunk
-        uint16_t const* xrow[NT];
-        bool live[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            live[n] = t0 + 8 * n + g < p.m;
-            xrow[n] = static_cast<uint16_t const*>(p.x) + static_cast<int64_t>(live[n] ? t0 + 8 * n + g : 0) * p.ldx + 8 * t;
-        }
-        uint4 xv[4][NT];
-        auto load_x = [&](int k0) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    xv[c][n] = live[n] && k0 + 32 * c < p.k ? *reinterpret_cast<uint4 const*>(xrow[n] + k0 + 32 * c)
-                                                            : make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < G; ++j) {
+                int const gi = min((k0 + 32 * GC * j) >> p.group_shift, p.groups - 1);
+                sc[j] = int4_scale(p, sbase0 + gi);
+                uint32_t const z = p.zero != nullptr ? p.zero[sbase0 + gi] : 8u;
+                zz[j] = ((kBf16 ? 0x4300u : 0x6400u) + z) * 0x10001u;
+            }
         };
         // ldmatrix: lanes 8 i .. 8 i + 7 give the rows of matrix i: rows 0-7 and 8-15 of a chunk, then of the next chunk
         uint32_t const mrow = ((lane >> 3) & 1) * 8 + (lane & 7);
-        uint32_t const mchunk = (warp & 1) * 4 + (lane >> 4);
-        uint32_t const moff = (warp >> 1) * 8192 + mrow * 128;
+        uint32_t const mchunk = (kq & 1) * 4 + (lane >> 4);
+        uint32_t const moff = (kq >> 1) * 8192 + rh * 4096 + mrow * 128;
         uint32_t const moff0 = moff + ((mchunk ^ (lane & 7)) << 4), moff2 = moff + (((mchunk + 2) ^ (lane & 7)) << 4);
 
-        load_scales(step0 * C::kStep + warp * 128);
-        griddep_wait();
-        load_x(step0 * C::kStep + warp * 128);
+        // B fragments: lane (g, t) takes row g of x and the elements 8 t .. 8 t + 7 of each chunk
+        uint32_t const xoff = C::kWeightBytes + kq * 2048 * NT + g * 128;
+        uint32_t const xoff0 = xoff + ((t ^ g) << 4), xoff1 = xoff + (((4 + t) ^ g) << 4);
+
+        load_scales(step0 * C::kStep + kq * 128);
         int stage = 0;
         uint32_t phase = 0;
         for (int st = step0; st < step1; ++st) {
-            int const k_next = (st + 1) * C::kStep + warp * 128;
-            uint32_t bx[4][NT][4];
+            int const k_next = (st + 1) * C::kStep + kq * 128;
+            float s_cur[G];
+            uint32_t z_cur[G];
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    uint4 const v = xv[c][n];
-                    bx[c][n][0] = __byte_perm(v.x, v.z, 0x5410);      // elements 0 and 4
-                    bx[c][n][1] = __byte_perm(v.x, v.z, 0x7632);      // 1 and 5
-                    bx[c][n][2] = __byte_perm(v.y, v.w, 0x5410);      // 2 and 6
-                    bx[c][n][3] = __byte_perm(v.y, v.w, 0x7632);      // 3 and 7
-                }
-            float s_cur[2][G];
-            uint32_t z_cur[2][G];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    s_cur[h][j] = sc[h][j];
-                    z_cur[h][j] = zz[h][j];
-                }
-            if (st + 1 < step1) {
-                load_x(k_next);
-                load_scales(k_next);
+            for (int j = 0; j < G; ++j) {
+                s_cur[j] = sc[j];
+                z_cur[j] = zz[j];
             }
+            if (st + 1 < step1) load_scales(k_next);
             if (!wait_or_abort(full_bar(stage), phase, abort_flag)) {
                 if (lane == 0) record_abort(FSO_DEV_WAIT_MMA_FULL, abort_flag);
                 break;
             }
             __syncwarp();
             uint32_t const sbase = base + stage * C::kStageBytes;
+            uint32_t w[2][2][4];      // [row tile][chunks 0, 1 or 2, 3]: row g and row g + 8 of the first, then of the second
 #pragma unroll
-            for (int rt = 0; rt < 4; ++rt) {
-                uint32_t w[2][4];
-                ldmatrix_x4(sbase + moff0 + rt * 2048, w[0]);
-                ldmatrix_x4(sbase + moff2 + rt * 2048, w[1]);
-                float acc[NT][4];
+            for (int rt = 0; rt < 2; ++rt) {
+                ldmatrix_x4(sbase + moff0 + rt * 2048, w[rt][0]);
+                ldmatrix_x4(sbase + moff2 + rt * 2048, w[rt][1]);
+            }
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    constexpr uint32_t kAll = 0xffffffffu;
-                    int const j = c / GC, src = (rt & 1) * 16 + g;
-                    uint32_t const z0 = __shfl_sync(kAll, z_cur[rt >> 1][j], src), z8 = __shfl_sync(kAll, z_cur[rt >> 1][j], src + 8);
-                    if (c % GC == 0) {
+            for (int j = 0; j < G; ++j) {
+                constexpr uint32_t kAll = 0xffffffffu;
+                float acc[2][NT][4] = {};
+                uint32_t zero2[2][2];
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-                    }
-                    uint32_t a[4], b[4];      // codes of row g and of row g + 8
-                    int4_unpack<kBf16>(w[c >> 1][2 * (c & 1)], z0, a);
-                    int4_unpack<kBf16>(w[c >> 1][2 * (c & 1) + 1], z8, b);
+                for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) zero2[rt][q] = __shfl_sync(kAll, z_cur[j], rt * 16 + q * 8 + g);
+#pragma unroll
+                for (int cc = 0; cc < GC; ++cc) {
+                    int const c = j * GC + cc;
+                    uint32_t bx[NT][4];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        mma_16x8x16<kBf16>(acc[n], a[0], b[0], a[1], b[1], bx[c][n][0], bx[c][n][1]);
-                        mma_16x8x16<kBf16>(acc[n], a[2], b[2], a[3], b[3], bx[c][n][2], bx[c][n][3]);
+                        uint4 v;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                     : "r"(sbase + (c & 1 ? xoff1 : xoff0) + (c >> 1) * 1024 * NT + n * 1024)
+                                     : "memory");
+                        bx[n][0] = __byte_perm(v.x, v.z, 0x5410);      // elements 0 and 4
+                        bx[n][1] = __byte_perm(v.x, v.z, 0x7632);      // 1 and 5
+                        bx[n][2] = __byte_perm(v.y, v.w, 0x5410);      // 2 and 6
+                        bx[n][3] = __byte_perm(v.y, v.w, 0x7632);      // 3 and 7
                     }
-                    if (c % GC == GC - 1) {
-                        float const s0 = __shfl_sync(kAll, s_cur[rt >> 1][j], src), s8 = __shfl_sync(kAll, s_cur[rt >> 1][j], src + 8);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            tot[rt][n][0] = fmaf(s0, acc[n][0], tot[rt][n][0]);
-                            tot[rt][n][1] = fmaf(s0, acc[n][1], tot[rt][n][1]);
-                            tot[rt][n][2] = fmaf(s8, acc[n][2], tot[rt][n][2]);
-                            tot[rt][n][3] = fmaf(s8, acc[n][3], tot[rt][n][3]);
-                        }
+                    for (int rt = 0; rt < 2; ++rt) {
+                        uint32_t a[4], b[4];      // row g, row g + 8
+                        int4_unpack<kBf16>(w[rt][c >> 1][2 * (c & 1)], zero2[rt][0], a);
+                        int4_unpack<kBf16>(w[rt][c >> 1][2 * (c & 1) + 1], zero2[rt][1], b);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_16x8x16<kBf16>(acc[rt][n], a[0], b[0], a[1], b[1], bx[n][0], bx[n][1]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_16x8x16<kBf16>(acc[rt][n], a[2], b[2], a[3], b[3], bx[n][2], bx[n][3]);
+                    }
+                }
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt) {
+                    float const s0 = __shfl_sync(kAll, s_cur[j], rt * 16 + g), s8 = __shfl_sync(kAll, s_cur[j], rt * 16 + 8 + g);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        tot[rt][n][0] = fmaf(s0, acc[rt][n][0], tot[rt][n][0]);
+                        tot[rt][n][1] = fmaf(s0, acc[rt][n][1], tot[rt][n][1]);
+                        tot[rt][n][2] = fmaf(s8, acc[rt][n][2], tot[rt][n][2]);
+                        tot[rt][n][3] = fmaf(s8, acc[rt][n][3], tot[rt][n][3]);
                     }
                 }
             }
@@ -304,7 +306,7 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
     }
 
     // ---------------------------------------------------------------------------------------- sums of the warps and slices
-    __syncthreads();      // every stage has been read: the ring becomes [warp][row of x][weight row]
+    __syncthreads();      // every stage has been read: the ring becomes [quarter][row of x][weight row]
     bool const failed = *abort_flag != 0;
     if (failed) {
         for (int i = 0; i < 200; ++i) __nanosleep(1000);      // copies in flight land before the memory is given up
@@ -312,18 +314,19 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
     }
     float* const red = reinterpret_cast<float*>(gbase);
     constexpr int kWarpFloats = 8 * NT * C::kRedStride;
-    static_assert(C::kWarps * kWarpFloats * 4 <= S * C::kStageBytes, "partial sums fit the ring");
+    static_assert(4 * kWarpFloats * 4 <= S * C::kStageBytes, "partial sums fit the ring");
     if (warp < C::kWarps) {
         int const g = lane >> 2, t = lane & 3;
 #pragma unroll
-        for (int rt = 0; rt < 4; ++rt)
+        for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    red[warp * kWarpFloats + (8 * n + 2 * t + (q & 1)) * C::kRedStride + rt * 16 + g + 8 * (q >> 1)] = tot[rt][n][q];
+                    red[kq * kWarpFloats + (8 * n + 2 * t + (q & 1)) * C::kRedStride + rh * 32 + rt * 16 + g + 8 * (q >> 1)] = tot[rt][n][q];
     }
     cluster_sync_all();
+    griddep_wait();      // the memory of the outputs may have been in use by the preceding kernel
     if (warp < C::kWarps && !failed) {
         int const cols = p.gated ? 32 : 64;
         int const rows = min(8 * NT, p.m - t0);
@@ -333,11 +336,11 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
             for (int r = 0; r < p.splits; ++r) {
                 uint32_t const peer = map_to_cta(red_addr + 4u * (row * C::kRedStride + col), r);
 #pragma unroll
-                for (int w = 0; w < C::kWarps; ++w) v += ld_cluster_f32(peer + 4u * (w * kWarpFloats));
+                for (int w = 0; w < 4; ++w) v += ld_cluster_f32(peer + 4u * (w * kWarpFloats));
             }
             return v;
         };
-        for (int i = rank * 128 + static_cast<int>(threadIdx.x); i < rows * cols; i += 128 * p.splits) {
+        for (int i = rank * 32 * C::kWarps + static_cast<int>(threadIdx.x); i < rows * cols; i += 32 * C::kWarps * p.splits) {
             int const row = i / cols, in_tile = i - row * cols;
             int const col = tile * cols + in_tile;
             if (col >= p.out_cols) continue;
@@ -424,16 +427,17 @@ inline void int4_slices(int64_t tiles, int sms, Int4Params& p)
 }
 
 template <bool kBf16, int NT, int GC>
-inline int launch_int4_inst(CUtensorMap const& lo, CUtensorMap const& hi, Int4Params const& p, dim3 grid, cudaStream_t stream)
+inline int launch_int4_inst(CUtensorMap const& lo, CUtensorMap const& hi, CUtensorMap const& mx, Int4Params const& p, dim3 grid, cudaStream_t stream)
 {
     static std::atomic<uint64_t> done{0};
+    using C = Int4Cfg<NT>;
     auto kernel = int4_rows_kernel<kBf16, NT, GC>;
-    int const rc = ensure_smem_attr(kernel, Int4Cfg::kSmemBytes, done);
+    int const rc = ensure_smem_attr(kernel, C::kSmemBytes, done);
     if (rc != 0) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(Int4Cfg::kThreads, 1, 1);
-    cfg.dynamicSmemBytes = Int4Cfg::kSmemBytes;
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -442,17 +446,17 @@ inline int launch_int4_inst(CUtensorMap const& lo, CUtensorMap const& hi, Int4Pa
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1 + pdl_attribute(&attr[1]);
-    FSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, lo, hi, p));
+    FSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, lo, hi, mx, p));
     return launch_status("int4_rows_kernel");
 }
 
 template <bool kBf16, int NT>
-inline int launch_int4_group(int group, CUtensorMap const& lo, CUtensorMap const& hi, Int4Params const& p, dim3 grid,
+inline int launch_int4_group(int group, CUtensorMap const& lo, CUtensorMap const& hi, CUtensorMap const& mx, Int4Params const& p, dim3 grid,
     cudaStream_t stream)
 {
-    return group == 32 ? launch_int4_inst<kBf16, NT, 1>(lo, hi, p, grid, stream)
-        : group == 64 ? launch_int4_inst<kBf16, NT, 2>(lo, hi, p, grid, stream)
-                      : launch_int4_inst<kBf16, NT, 4>(lo, hi, p, grid, stream);
+    return group == 32 ? launch_int4_inst<kBf16, NT, 1>(lo, hi, mx, p, grid, stream)
+        : group == 64 ? launch_int4_inst<kBf16, NT, 2>(lo, hi, mx, p, grid, stream)
+                      : launch_int4_inst<kBf16, NT, 4>(lo, hi, mx, p, grid, stream);
 }
 
 // p: everything but the fields that are derived here.
@@ -461,21 +465,23 @@ inline int launch_int4(Int4Params p, const uint8_t* codes, int64_t group, bool b
     p.group_shift = 0;
     while ((1ll << p.group_shift) < group) ++p.group_shift;
     p.groups = p.k >> p.group_shift;
-    p.steps = (p.k + Int4Cfg::kStep - 1) / Int4Cfg::kStep;
+    p.steps = (p.k + Int4Cfg<1>::kStep - 1) / Int4Cfg<1>::kStep;
     int const per_tile = p.gated ? 32 : 64;
     int const tiles = (p.out_cols + per_tile - 1) / per_tile;
     int4_slices(tiles, sm_count(), p);
-    CUtensorMap lo, hi;
+    int const nt = p.m <= 8 ? 1 : 2;
+    CUtensorMap lo, hi, mx;
     int rc = make_codes_map(&lo, codes, p.out_cols, p.k, 32);
     if (rc != 0) return rc;
     hi = lo;
     if (p.gated) rc = make_codes_map(&hi, codes + static_cast<int64_t>(p.out_cols) * (p.k / 2), p.out_cols, p.k, 32);
     if (rc != 0) return rc;
-    int const nt = p.m <= 8 ? 1 : 2;
+    rc = make_map16(&mx, p.x, p.m, p.k, p.ldx, 8 * nt);
+    if (rc != 0) return rc;
     dim3 const grid(static_cast<unsigned>(tiles * p.splits), static_cast<unsigned>((p.m + 8 * nt - 1) / (8 * nt)));
     int const gi = static_cast<int>(std::min<int64_t>(group, 128));
-    if (bf16) return nt == 1 ? launch_int4_group<true, 1>(gi, lo, hi, p, grid, stream) : launch_int4_group<true, 2>(gi, lo, hi, p, grid, stream);
-    return nt == 1 ? launch_int4_group<false, 1>(gi, lo, hi, p, grid, stream) : launch_int4_group<false, 2>(gi, lo, hi, p, grid, stream);
+    if (bf16) return nt == 1 ? launch_int4_group<true, 1>(gi, lo, hi, mx, p, grid, stream) : launch_int4_group<true, 2>(gi, lo, hi, mx, p, grid, stream);
+    return nt == 1 ? launch_int4_group<false, 1>(gi, lo, hi, mx, p, grid, stream) : launch_int4_group<false, 2>(gi, lo, hi, mx, p, grid, stream);
 }
 
 }  // namespace fso

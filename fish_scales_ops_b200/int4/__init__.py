@@ -19,7 +19,6 @@ import torch
 
 from .. import _ops
 from .._arch import SERVED_MAJOR, arch_label, device_arch
-from .._lib import eager_or_op
 
 __all__ = ["ACTIVATIONS", "GROUP_SIZES", "Int4Weight", "prepare_weight", "quantize_weight", "linear", "gated_linear"]
 
@@ -77,15 +76,28 @@ def _check_weight(op: str, codes, scale, zero) -> None:
 
 
 def _check_x(op: str, x, codes) -> None:
-    k = 2 * int(codes.shape[1])
+    k = 2 * codes.shape[1]
     if x.dim() != 2 or x.shape[1] != k:
         raise ValueError(f"{op}: x must be [..., {k}] (K = in_features), got {tuple(x.shape)}")
     if x.dtype not in _ops.DTYPES_16:
         raise ValueError(f"{op}: x must be bf16 or fp16, got {x.dtype}")
-    if x.device != codes.device:
-        raise ValueError(f"{op}: x lives on {x.device}, the weight on {codes.device}")
+    if not x.is_cuda or x.get_device() != codes.get_device():
+        raise ValueError(f"{op}: x lives on {x.device}, the weight on {codes.device}; both must be on one CUDA device")
     if x.shape[0] > _MAX_ROWS:
         raise ValueError(f"{op}: {int(x.shape[0])} rows of x; at most {_MAX_ROWS} are served")
+
+
+def _check_bias(op: str, bias, x, n: int) -> None:
+    if bias.dtype != x.dtype or tuple(bias.shape) != (n,) or bias.device != x.device or not bias.is_contiguous():
+        raise ValueError(f"{op}: bias must be a contiguous {x.dtype} [{n}] tensor on {x.device}, got {bias.dtype} "
+                         f"{tuple(bias.shape)} on {bias.device}")
+
+
+def _check_gate(op: str, codes, activation) -> None:
+    if activation not in _ops.GATE_ACTIVATIONS:
+        raise ValueError(f"{op}: unknown activation {activation!r}; the activations are {', '.join(ACTIVATIONS)}")
+    if codes.shape[0] % 2 != 0:
+        raise ValueError(f"{op}: a gate_up weight has an even number of rows, got {int(codes.shape[0])}")
 
 
 def _need_arch(op: str) -> None:
@@ -107,27 +119,24 @@ def _aligned(t):
 
 # ------------------------------------------------------------------------------------------------ custom ops
 
+# The ops check all their tensors. The public functions below check a handle's tensors when they make the handle, not at
+# each call: the checks would take longer than a decode-sized kernel runs.
+
 def _int4_linear_body(x, codes, scale, zero=None, bias=None):
     op = f"fish_scales_ops::int4_linear ({arch_label(device_arch())})"
     _check_weight(op, codes, scale, zero)
     _check_x(op, x, codes)
-    n = int(codes.shape[0])
-    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,) or bias.device != x.device
-                             or not bias.is_contiguous()):
-        raise ValueError(f"{op}: bias must be a contiguous {x.dtype} [{n}] tensor on {x.device}, got {bias.dtype} "
-                         f"{tuple(bias.shape)} on {bias.device}")
+    if bias is not None:
+        _check_bias(op, bias, x, int(codes.shape[0]))
     _need_arch(op)
     return _ops.int4_linear(x, codes, scale, zero, bias)
 
 
 def _int4_gated_linear_body(x, codes, scale, zero, activation):
     op = f"fish_scales_ops::int4_gated_linear ({arch_label(device_arch())})"
-    if activation not in _ops.GATE_ACTIVATIONS:
-        raise ValueError(f"{op}: unknown activation {activation!r}; the activations are {', '.join(ACTIVATIONS)}")
     _check_weight(op, codes, scale, zero)
+    _check_gate(op, codes, activation)
     _check_x(op, x, codes)
-    if codes.shape[0] % 2 != 0:
-        raise ValueError(f"{op}: a gate_up weight has an even number of rows, got {int(codes.shape[0])}")
     _need_arch(op)
     return _ops.int4_gated_linear(x, codes, scale, zero, _ops.GATE_ACTIVATIONS[activation])
 
@@ -214,8 +223,13 @@ def linear(x: torch.Tensor, weight: Int4Weight, *, bias: Optional[torch.Tensor] 
     for the few of a decode step. Nothing synchronizes; the call can be captured into a CUDA graph after one eager call
     of the same shape."""
     x2 = _flatten(x, weight, "fso.int4.linear")
-    y = eager_or_op(_int4_linear_body, torch.ops.fish_scales_ops.int4_linear, x2, weight.codes, weight.scale, weight.zero,
-                    bias)
+    if torch.compiler.is_compiling():
+        y = torch.ops.fish_scales_ops.int4_linear(x2, weight.codes, weight.scale, weight.zero, bias)
+    else:
+        _check_x("fso.int4.linear", x2, weight.codes)
+        if bias is not None:
+            _check_bias("fso.int4.linear", bias, x2, weight.out_features)
+        y = _ops.int4_linear(x2, weight.codes, weight.scale, weight.zero, bias)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.out_features)
 
 
@@ -224,6 +238,10 @@ def gated_linear(x: torch.Tensor, gate_up: Int4Weight, *, activation: str = "sil
     ``fso.ffn.gated_linear``): ``x [..., K]`` bf16 or fp16, result ``[..., N/2]`` of the same type. ``activation``:
     ``"silu"``, ``"gelu"`` (erf) or ``"gelu_tanh"``. Otherwise as :func:`linear`."""
     x2 = _flatten(x, gate_up, "fso.int4.gated_linear")
-    h = eager_or_op(_int4_gated_linear_body, torch.ops.fish_scales_ops.int4_gated_linear, x2, gate_up.codes, gate_up.scale,
-                    gate_up.zero, activation)
+    if torch.compiler.is_compiling():
+        h = torch.ops.fish_scales_ops.int4_gated_linear(x2, gate_up.codes, gate_up.scale, gate_up.zero, activation)
+    else:
+        _check_gate("fso.int4.gated_linear", gate_up.codes, activation)
+        _check_x("fso.int4.gated_linear", x2, gate_up.codes)
+        h = _ops.int4_gated_linear(x2, gate_up.codes, gate_up.scale, gate_up.zero, _ops.GATE_ACTIVATIONS[activation])
     return h if x.dim() == 2 else h.reshape(*x.shape[:-1], gate_up.out_features // 2)
