@@ -393,8 +393,13 @@ def gated_linear_backward(dh, x, gate_up, hi, lo, activation: int, need_x: bool,
     return dx, dw
 
 
+def int4_half_cols(rows: int) -> int:
+    """Columns from one half of a 4-bit weight's rows to the other in its scales and zero points."""
+    return _align((rows + 1) // 2, 16)
+
+
 def int4_linear(x, codes, scale, zero, bias):
-    """x [M, K] and a 4-bit weight of N rows -> y [M, N]."""
+    """x [M, K] and a 4-bit weight of N rows (scale and zero [K/group, 2 * half]) -> y [M, N]."""
     m, k = x.shape
     n = codes.shape[0]
     y = x.new_empty((m, n))
@@ -402,7 +407,7 @@ def int4_linear(x, codes, scale, zero, bias):
         x, ldx = rows_in_place(x)
         rc = call_on(x, lib().fso_int4_linear, x.data_ptr(), ldx, codes.data_ptr(), scale.data_ptr(),
                      None if zero is None else zero.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), m, n,
-                     k, k // scale.shape[1], DTYPES_16[x.dtype], _SCALE_DTYPES[scale.dtype])
+                     k, k // scale.shape[0], DTYPES_16[x.dtype], _SCALE_DTYPES[scale.dtype])
         if rc != 0:
             check(rc, "fso_int4_linear")
     return y
@@ -416,7 +421,7 @@ def int4_gated_linear(x, codes, scale, zero, activation: int):
     if m > 0:
         x, ldx = rows_in_place(x)
         rc = call_on(x, lib().fso_int4_gated_linear, x.data_ptr(), ldx, codes.data_ptr(), scale.data_ptr(),
-                     None if zero is None else zero.data_ptr(), h.data_ptr(), m, inter, k, k // scale.shape[1],
+                     None if zero is None else zero.data_ptr(), h.data_ptr(), m, inter, k, k // scale.shape[0],
                      DTYPES_16[x.dtype], _SCALE_DTYPES[scale.dtype], activation)
         if rc != 0:
             check(rc, "fso_int4_gated_linear")
@@ -424,12 +429,13 @@ def int4_gated_linear(x, codes, scale, zero, activation: int):
 
 
 def int4_quantize(w, group: int, zero_point: bool, scale_dtype):
-    """16-bit w [N, K] -> (codes uint8 [N, K/2], scale [N, K/group], zero uint8 [N, K/group] or None)."""
+    """16-bit w [N, K] -> (codes uint8 [N, K/2], scale [K/group, 2 * half], zero uint8 like it or None)."""
     n, k = int(w.shape[0]), int(w.shape[1])
     with on_device(w.device):
         codes = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
-        scale = torch.empty((n, k // group), dtype=scale_dtype, device=w.device)
-        zero = torch.empty((n, k // group), dtype=torch.uint8, device=w.device) if zero_point else None
+        cols = 2 * int4_half_cols(n)
+        scale = torch.zeros((k // group, cols), dtype=scale_dtype, device=w.device)
+        zero = torch.zeros((k // group, cols), dtype=torch.uint8, device=w.device) if zero_point else None
         check(lib().fso_int4_quantize(ptr(w), ptr(codes), ptr(scale), ptr(zero), n, k, int(group), DTYPES_16[w.dtype],
                                       _SCALE_DTYPES[scale_dtype], stream_ptr()), "fso_int4_quantize")
     return codes, scale, zero

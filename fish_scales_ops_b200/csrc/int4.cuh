@@ -16,14 +16,14 @@ namespace fso {
 struct Int4Params {
     const void* x;         // 16 bit [m, ldx]
     int64_t ldx;
-    const void* scale;     // [rows, groups]
     int scale_type;        // 0 bf16, 1 fp16, 2 fp32
-    const uint8_t* zero;   // [rows, groups], or nullptr: 8
+    int has_zero;          // otherwise 8
     const void* bias;      // [out_cols], 16 bit like x, or nullptr
     void* out;             // 16 bit [m, out_cols]
     int m, k;
     int group_shift;       // log2 of the group size
-    int groups;            // groups of a row
+    int rows0, rows1;      // rows of the first and of the second half of the weight
+    int half_cols;         // columns of scale and zero from one half to the other
     int out_cols;          // rows of the weight, or half of them when gated
     int gated;
     int act;
@@ -31,13 +31,6 @@ struct Int4Params {
     int steps_per_slice;
     int splits;            // slices of the contraction = CTAs of a cluster
 };
-
-__device__ __forceinline__ float int4_scale(Int4Params const& p, int64_t i)
-{
-    if (p.scale_type == 0) return load16<true>(p.scale, i);
-    if (p.scale_type == 1) return load16<false>(p.scale, i);
-    return static_cast<float const*>(p.scale)[i];
-}
 
 // Eight codes of a word to the eight 16-bit numbers code - zero, exactly: a code in the low bits of the mantissa of 128
 // (bf16) or 1024 (fp16) is 128 + code, and taking away 128 + zero is exact. Register i gets the codes i and i + 4, which
@@ -90,17 +83,21 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
 
 template <int NT>
 struct Int4Cfg {
-    static constexpr int kRows = 64;             // weight rows of a CTA (gated: 32 of each half)
+    static constexpr int kRT = 2;                // 16-row tiles of a warp
+    static constexpr int kRows = 64;             // weight rows of a CTA, 32 of each half of the weight
     static constexpr int kStep = 512;            // of the contraction in a stage, 128 for a warp
-    static constexpr int kWarps = 8;             // four along the contraction, two along the rows
+    static constexpr int kWarps = 16 / kRT;             // four along the contraction, two along the rows
     static constexpr int kThreads = 32 * kWarps + 32;
-    static constexpr int kStages = NT == 1 ? 4 : 3;
+    static constexpr int kStages = NT == 1 ? 3 : 2;
+    static constexpr int kBlocks = 2;
     static constexpr int kWeightBytes = kRows * kStep / 2;
     static constexpr int kXBytes = 8 * NT * kStep * 2;
-    static constexpr int kStageBytes = kWeightBytes + kXBytes;
+    static constexpr int kScaleOff = kWeightBytes + kXBytes;                  // [half][group][32 rows], at most 16 groups
+    static constexpr int kZeroOff = kScaleOff + 2 * 16 * 32 * 4;
+    static constexpr int kStageBytes = kZeroOff + 2 * 16 * 32;                // 16 KB of codes, x, 4 KB + 1 KB
     static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
     static constexpr int kRedStride = kRows + 4; // floats between the rows of x in the partial sums: lanes hit 32 banks
-    static_assert(2 * (kSmemBytes + 1024) <= 227 * 1024, "two CTAs per SM");
+    static_assert(kBlocks * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
 };
 
 // The few rows of x of a decode step (at most 8 * NT in a CTA) against 64 rows of the weight.
@@ -117,9 +114,10 @@ struct Int4Cfg {
 //
 // GC: 32-wide chunks of a group inside the 128 of a warp (4 for groups of 128 and more).
 template <bool kBf16, int NT, int GC>
-__global__ void __launch_bounds__(Int4Cfg<NT>::kThreads, 2)
+__global__ void __launch_bounds__(Int4Cfg<NT>::kThreads, Int4Cfg<NT>::kBlocks)
 int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ CUtensorMap tm_hi,
-    const __grid_constant__ CUtensorMap tm_x, const Int4Params p)
+    const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_scale,
+    const __grid_constant__ CUtensorMap tm_zero, const Int4Params p)
 {
     using C = Int4Cfg<NT>;
     constexpr int S = C::kStages;
@@ -152,21 +150,30 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
     __syncthreads();
     griddep_launch_dependents();
 
-    int const kq = warp & 3, rh = (warp >> 2) & 1;      // this warp's quarter of a step and half of the rows
-    float tot[2][NT][4] = {};
+    constexpr int RT = C::kRT;
+    int const kq = warp & 3, rh = RT == 4 ? 0 : (warp >> 2) & 1;      // this warp's quarter of a step and half of the rows
+    float tot[RT][NT][4] = {};
     if (warp == C::kWarps) {
         // -------------------------------------------------------------------------------- weight stream (immutable bytes:
         // it starts under the preceding kernel)
         if (elect_one()) {
-            int const row_lo = tile * (p.gated ? 32 : 64);
-            int const row_hi = p.gated ? row_lo : row_lo + 32;
+            int const row0 = tile * 32;
+            int const box_groups = max(1, C::kStep >> p.group_shift);
+            uint32_t const scale_bytes = box_groups * 32 * (p.scale_type == 2 ? 4 : 2), zero_bytes = box_groups * 32;
+            uint32_t const bytes = C::kWeightBytes + C::kXBytes + 2 * scale_bytes + (p.has_zero ? 2 * zero_bytes : 0);
             auto load_weight = [&](int stage, int st) {
                 uint32_t const fb = full_bar(stage), dst = base + stage * C::kStageBytes;
-                mbar_expect_tx(fb, C::kStageBytes);
+                int const g0 = (st * C::kStep) >> p.group_shift;
+                mbar_expect_tx(fb, bytes);
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    tma_load_2d(dst + b * 8192, &tm_lo, fb, st * (C::kStep / 2) + b * 128, row_lo);
-                    tma_load_2d(dst + b * 8192 + 4096, &tm_hi, fb, st * (C::kStep / 2) + b * 128, row_hi);
+                    tma_load_2d(dst + b * 8192, &tm_lo, fb, st * (C::kStep / 2) + b * 128, row0);
+                    tma_load_2d(dst + b * 8192 + 4096, &tm_hi, fb, st * (C::kStep / 2) + b * 128, row0);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    tma_load_2d(dst + C::kScaleOff + h * 2048, &tm_scale, fb, row0 + h * p.half_cols, g0);
+                    if (p.has_zero) tma_load_2d(dst + C::kZeroOff + h * 512, &tm_zero, fb, row0 + h * p.half_cols, g0);
                 }
             };
             auto load_x = [&](int stage, int st) {
@@ -198,21 +205,6 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
         __syncwarp();
     } else {
         int const g = lane >> 2, t = lane & 3;
-        // lane l looks after the scales of row l of the warp's 32; rows past the last one borrow its scales
-        int const srow = p.gated ? min(tile * 32 + lane, p.out_cols - 1) + rh * p.out_cols
-                                 : min(tile * 64 + rh * 32 + lane, p.out_cols - 1);
-        int64_t const sbase0 = static_cast<int64_t>(srow) * p.groups;
-        float sc[G];
-        uint32_t zz[G];
-        auto load_scales = [&](int k0) {
-#pragma unroll
-            for (int j = 0; j < G; ++j) {
-                int const gi = min((k0 + 32 * GC * j) >> p.group_shift, p.groups - 1);
-                sc[j] = int4_scale(p, sbase0 + gi);
-                uint32_t const z = p.zero != nullptr ? p.zero[sbase0 + gi] : 8u;
-                zz[j] = ((kBf16 ? 0x4300u : 0x6400u) + z) * 0x10001u;
-            }
-        };
         // ldmatrix: lanes 8 i .. 8 i + 7 give the rows of matrix i: rows 0-7 and 8-15 of a chunk, then of the next chunk
         uint32_t const mrow = ((lane >> 3) & 1) * 8 + (lane & 7);
         uint32_t const mchunk = (kq & 1) * 4 + (lane >> 4);
@@ -223,40 +215,50 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
         uint32_t const xoff = C::kWeightBytes + kq * 2048 * NT + g * 128;
         uint32_t const xoff0 = xoff + ((t ^ g) << 4), xoff1 = xoff + (((4 + t) ^ g) << 4);
 
-        load_scales(step0 * C::kStep + kq * 128);
+        // scales and zero points of a row and group: lane (g, t) needs those of rows g and g + 8 of each 16
+        uint32_t const scale_width = p.scale_type == 2 ? 4 : 2;
+        int const group0 = (kq * 128) >> p.group_shift;      // of this warp inside a stage (0 where a group spans stages)
+        auto scale_of = [&](uint32_t sbase, int row, int j) -> float {      // row 0..63 of the tile
+            uint32_t const at = sbase + C::kScaleOff + (row >> 5) * 2048 + ((group0 + j) * 32 + (row & 31)) * scale_width;
+            if (p.scale_type == 2) {
+                float v;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+                return v;
+            }
+            uint16_t v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+            return p.scale_type == 0 ? __uint_as_float(static_cast<uint32_t>(v) << 16) : __half2float(__ushort_as_half(v));
+        };
+        auto zero_of = [&](uint32_t sbase, int row, int j) -> uint32_t {
+            uint32_t z = 8;
+            if (p.has_zero)
+                asm volatile("ld.shared.u8 %0, [%1];"
+                             : "=r"(z) : "r"(sbase + C::kZeroOff + (row >> 5) * 512 + (group0 + j) * 32 + (row & 31)) : "memory");
+            return ((kBf16 ? 0x4300u : 0x6400u) + z) * 0x10001u;
+        };
         int stage = 0;
         uint32_t phase = 0;
         for (int st = step0; st < step1; ++st) {
-            int const k_next = (st + 1) * C::kStep + kq * 128;
-            float s_cur[G];
-            uint32_t z_cur[G];
-#pragma unroll
-            for (int j = 0; j < G; ++j) {
-                s_cur[j] = sc[j];
-                z_cur[j] = zz[j];
-            }
-            if (st + 1 < step1) load_scales(k_next);
             if (!wait_or_abort(full_bar(stage), phase, abort_flag)) {
                 if (lane == 0) record_abort(FSO_DEV_WAIT_MMA_FULL, abort_flag);
                 break;
             }
             __syncwarp();
             uint32_t const sbase = base + stage * C::kStageBytes;
-            uint32_t w[2][2][4];      // [row tile][chunks 0, 1 or 2, 3]: row g and row g + 8 of the first, then of the second
+            uint32_t w[RT][2][4];      // [row tile][chunks 0, 1 or 2, 3]: row g and row g + 8 of the first, then of the second
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
+            for (int rt = 0; rt < RT; ++rt) {
                 ldmatrix_x4(sbase + moff0 + rt * 2048, w[rt][0]);
                 ldmatrix_x4(sbase + moff2 + rt * 2048, w[rt][1]);
             }
 #pragma unroll
             for (int j = 0; j < G; ++j) {
-                constexpr uint32_t kAll = 0xffffffffu;
-                float acc[2][NT][4] = {};
-                uint32_t zero2[2][2];
+                float acc[RT][NT][4] = {};
+                uint32_t zero2[RT][2];
 #pragma unroll
-                for (int rt = 0; rt < 2; ++rt)
+                for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) zero2[rt][q] = __shfl_sync(kAll, z_cur[j], rt * 16 + q * 8 + g);
+                    for (int q = 0; q < 2; ++q) zero2[rt][q] = zero_of(sbase, rh * 32 + rt * 16 + q * 8 + g, j);
 #pragma unroll
                 for (int cc = 0; cc < GC; ++cc) {
                     int const c = j * GC + cc;
@@ -274,7 +276,7 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
                         bx[n][3] = __byte_perm(v.y, v.w, 0x7632);      // 3 and 7
                     }
 #pragma unroll
-                    for (int rt = 0; rt < 2; ++rt) {
+                    for (int rt = 0; rt < RT; ++rt) {
                         uint32_t a[4], b[4];      // row g, row g + 8
                         int4_unpack<kBf16>(w[rt][c >> 1][2 * (c & 1)], zero2[rt][0], a);
                         int4_unpack<kBf16>(w[rt][c >> 1][2 * (c & 1) + 1], zero2[rt][1], b);
@@ -285,8 +287,8 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
                     }
                 }
 #pragma unroll
-                for (int rt = 0; rt < 2; ++rt) {
-                    float const s0 = __shfl_sync(kAll, s_cur[j], rt * 16 + g), s8 = __shfl_sync(kAll, s_cur[j], rt * 16 + 8 + g);
+                for (int rt = 0; rt < RT; ++rt) {
+                    float const s0 = scale_of(sbase, rh * 32 + rt * 16 + g, j), s8 = scale_of(sbase, rh * 32 + rt * 16 + 8 + g, j);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         tot[rt][n][0] = fmaf(s0, acc[rt][n][0], tot[rt][n][0]);
@@ -318,14 +320,15 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
     if (warp < C::kWarps) {
         int const g = lane >> 2, t = lane & 3;
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     red[kq * kWarpFloats + (8 * n + 2 * t + (q & 1)) * C::kRedStride + rh * 32 + rt * 16 + g + 8 * (q >> 1)] = tot[rt][n][q];
     }
-    cluster_sync_all();
+    if (p.splits > 1) cluster_sync_all();
+    else __syncthreads();
     griddep_wait();      // the memory of the outputs may have been in use by the preceding kernel
     if (warp < C::kWarps && !failed) {
         int const cols = p.gated ? 32 : 64;
@@ -333,6 +336,11 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
         uint32_t const red_addr = smem_u32(red);
         auto sum_of = [&](int row, int col) {
             float v = 0.f;
+            if (p.splits == 1) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) v += red[w * kWarpFloats + row * C::kRedStride + col];
+                return v;
+            }
             for (int r = 0; r < p.splits; ++r) {
                 uint32_t const peer = map_to_cta(red_addr + 4u * (row * C::kRedStride + col), r);
 #pragma unroll
@@ -342,8 +350,9 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
         };
         for (int i = rank * 32 * C::kWarps + static_cast<int>(threadIdx.x); i < rows * cols; i += 32 * C::kWarps * p.splits) {
             int const row = i / cols, in_tile = i - row * cols;
-            int const col = tile * cols + in_tile;
-            if (col >= p.out_cols) continue;
+            int const half = in_tile >> 5, in_half = tile * 32 + (in_tile & 31);      // row of the half
+            if (in_half >= (half ? p.rows1 : p.rows0)) continue;
+            int const col = half * p.rows0 + in_half;
             float v = sum_of(row, in_tile);
             if (p.gated) v = gate_value(v, p.act) * sum_of(row, in_tile + 32);
             else if (p.bias != nullptr) v += load16<kBf16>(p.bias, col);
@@ -351,7 +360,7 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
         }
     }
     __syncwarp();
-    cluster_sync_all();      // no CTA leaves while another may still read its sums
+    if (p.splits > 1) cluster_sync_all();      // no CTA leaves while another may still read its sums
 }
 
 // ------------------------------------------------------------------------------------------------ 16-bit weight -> 4 bits
@@ -368,7 +377,7 @@ __device__ __forceinline__ float stored_scale(float v, int type)
 
 template <bool kBf16>
 __global__ void int4_quantize_kernel(const uint4* __restrict__ w, uint32_t* __restrict__ codes, void* __restrict__ scale,
-    int scale_type, uint8_t* __restrict__ zero, int64_t vectors, int lanes)
+    int scale_type, uint8_t* __restrict__ zero, int64_t vectors, int lanes, int64_t rows0, int64_t half_cols, int groups)
 {
     int64_t const i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     bool const live = i < vectors;      // groups are whole: all lanes of one are live or none is
@@ -402,7 +411,8 @@ __global__ void int4_quantize_kernel(const uint4* __restrict__ w, uint32_t* __re
     if (!live) return;
     codes[i] = packed;
     if (i % lanes == 0) {
-        int64_t const g = i / lanes;
+        int64_t const row_group = i / lanes, row = row_group / groups;
+        int64_t const g = (row_group - row * groups) * 2 * half_cols + (row < rows0 ? row : half_cols + row - rows0);
         if (scale_type == 0) store16<true>(scale, g, step);
         else if (scale_type == 1) store16<false>(scale, g, step);
         else static_cast<float*>(scale)[g] = step;
@@ -427,7 +437,7 @@ inline void int4_slices(int64_t tiles, int sms, Int4Params& p)
 }
 
 template <bool kBf16, int NT, int GC>
-inline int launch_int4_inst(CUtensorMap const& lo, CUtensorMap const& hi, CUtensorMap const& mx, Int4Params const& p, dim3 grid, cudaStream_t stream)
+inline int launch_int4_inst(CUtensorMap const (&maps)[5], Int4Params const& p, dim3 grid, cudaStream_t stream)
 {
     static std::atomic<uint64_t> done{0};
     using C = Int4Cfg<NT>;
@@ -446,42 +456,74 @@ inline int launch_int4_inst(CUtensorMap const& lo, CUtensorMap const& hi, CUtens
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1 + pdl_attribute(&attr[1]);
-    FSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, lo, hi, mx, p));
+    FSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], maps[4], p));
     return launch_status("int4_rows_kernel");
 }
 
 template <bool kBf16, int NT>
-inline int launch_int4_group(int group, CUtensorMap const& lo, CUtensorMap const& hi, CUtensorMap const& mx, Int4Params const& p, dim3 grid,
+inline int launch_int4_group(int group, CUtensorMap const (&maps)[5], Int4Params const& p, dim3 grid,
     cudaStream_t stream)
 {
-    return group == 32 ? launch_int4_inst<kBf16, NT, 1>(lo, hi, mx, p, grid, stream)
-        : group == 64 ? launch_int4_inst<kBf16, NT, 2>(lo, hi, mx, p, grid, stream)
-                      : launch_int4_inst<kBf16, NT, 4>(lo, hi, mx, p, grid, stream);
+    return group == 32 ? launch_int4_inst<kBf16, NT, 1>(maps, p, grid, stream)
+        : group == 64 ? launch_int4_inst<kBf16, NT, 2>(maps, p, grid, stream)
+                      : launch_int4_inst<kBf16, NT, 4>(maps, p, grid, stream);
 }
 
-// p: everything but the fields that are derived here.
-inline int launch_int4(Int4Params p, const uint8_t* codes, int64_t group, bool bf16, cudaStream_t stream)
+// Tensor map of scale or zero [groups, 2 * half_cols] in boxes of 32 rows of the weight x box_groups.
+inline int make_steps_map(CUtensorMap* map, const void* base, int64_t groups, int64_t half_cols, int width, int box_groups)
+{
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) {
+        set_error("cuTensorMapEncodeTiled is not available from this driver");
+        return FSO_ERR_UNSUPPORTED;
+    }
+    cuuint64_t const dims[2] = {static_cast<cuuint64_t>(2 * half_cols), static_cast<cuuint64_t>(groups)};
+    cuuint64_t const strides[1] = {static_cast<cuuint64_t>(2 * half_cols * width)};
+    cuuint32_t const box[2] = {32u, static_cast<cuuint32_t>(box_groups)};
+    cuuint32_t const estr[2] = {1u, 1u};
+    CUtensorMapDataType const type = width == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : width == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                                                                          : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    CUresult const r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed with CUresult %d (scales, %lld groups)", static_cast<int>(r),
+            static_cast<long long>(groups));
+        return FSO_ERR_INTERNAL;
+    }
+    return 0;
+}
+
+inline int64_t int4_half_cols(int64_t rows) { return ((rows + 1) / 2 + 15) / 16 * 16; }
+
+// p: x, ldx, scale_type, bias, out, m, k, out_cols, gated and act; the rest is derived here.
+inline int launch_int4(Int4Params p, int64_t rows, const uint8_t* codes, const void* scale, const void* zero, int64_t group,
+    bool bf16, cudaStream_t stream)
 {
     p.group_shift = 0;
     while ((1ll << p.group_shift) < group) ++p.group_shift;
-    p.groups = p.k >> p.group_shift;
+    p.has_zero = zero != nullptr;
+    p.rows0 = static_cast<int>((rows + 1) / 2);
+    p.rows1 = static_cast<int>(rows - p.rows0);
+    p.half_cols = static_cast<int>(int4_half_cols(rows));
     p.steps = (p.k + Int4Cfg<1>::kStep - 1) / Int4Cfg<1>::kStep;
-    int const per_tile = p.gated ? 32 : 64;
-    int const tiles = (p.out_cols + per_tile - 1) / per_tile;
+    int const tiles = (p.rows0 + 31) / 32;
     int4_slices(tiles, sm_count(), p);
     int const nt = p.m <= 8 ? 1 : 2;
-    CUtensorMap lo, hi, mx;
-    int rc = make_codes_map(&lo, codes, p.out_cols, p.k, 32);
-    if (rc != 0) return rc;
-    hi = lo;
-    if (p.gated) rc = make_codes_map(&hi, codes + static_cast<int64_t>(p.out_cols) * (p.k / 2), p.out_cols, p.k, 32);
-    if (rc != 0) return rc;
-    rc = make_map16(&mx, p.x, p.m, p.k, p.ldx, 8 * nt);
+    int const box_groups = static_cast<int>(std::max<int64_t>(1, Int4Cfg<1>::kStep / group));
+    int64_t const groups = p.k >> p.group_shift;
+    CUtensorMap maps[5];
+    int rc = make_codes_map(&maps[0], codes, p.rows0, p.k, 32);
+    maps[1] = maps[0];      // a weight of one row has no second half: what is read in its place goes nowhere
+    if (rc == 0 && p.rows1 > 0) rc = make_codes_map(&maps[1], codes + static_cast<int64_t>(p.rows0) * (p.k / 2), p.rows1, p.k, 32);
+    if (rc == 0) rc = make_map16(&maps[2], p.x, p.m, p.k, p.ldx, 8 * nt);
+    if (rc == 0) rc = make_steps_map(&maps[3], scale, groups, p.half_cols, p.scale_type == 2 ? 4 : 2, box_groups);
+    maps[4] = maps[3];
+    if (rc == 0 && p.has_zero) rc = make_steps_map(&maps[4], zero, groups, p.half_cols, 1, box_groups);
     if (rc != 0) return rc;
     dim3 const grid(static_cast<unsigned>(tiles * p.splits), static_cast<unsigned>((p.m + 8 * nt - 1) / (8 * nt)));
     int const gi = static_cast<int>(std::min<int64_t>(group, 128));
-    if (bf16) return nt == 1 ? launch_int4_group<true, 1>(gi, lo, hi, mx, p, grid, stream) : launch_int4_group<true, 2>(gi, lo, hi, mx, p, grid, stream);
-    return nt == 1 ? launch_int4_group<false, 1>(gi, lo, hi, mx, p, grid, stream) : launch_int4_group<false, 2>(gi, lo, hi, mx, p, grid, stream);
+    if (bf16) return nt == 1 ? launch_int4_group<true, 1>(gi, maps, p, grid, stream) : launch_int4_group<true, 2>(gi, maps, p, grid, stream);
+    return nt == 1 ? launch_int4_group<false, 1>(gi, maps, p, grid, stream) : launch_int4_group<false, 2>(gi, maps, p, grid, stream);
 }
 
 }  // namespace fso

@@ -754,7 +754,7 @@ int fso_gated_linear_backward(const void* dh, int64_t ldh, const void* x, int64_
 }
 
 static int check_int4(const char* op, int64_t m, int64_t rows, int64_t k, int64_t group, int64_t dtype, int64_t scale_dtype,
-    const void* x, int64_t ldx, const void* codes, const void* scale, const void* out)
+    const void* x, int64_t ldx, const void* codes, const void* scale, const void* zero, const void* out)
 {
     FSO_REQUIRE(m >= 0 && rows > 0 && k > 0, "%s: M >= 0, rows > 0 and K > 0 required", op);
     FSO_REQUIRE(group >= 32 && (group & (group - 1)) == 0 && k % group == 0,
@@ -766,7 +766,8 @@ static int check_int4(const char* op, int64_t m, int64_t rows, int64_t k, int64_
     if (m == 0) return 0;
     FSO_REQUIRE(x && codes && scale && out, "%s: NULL pointer", op);
     FSO_REQUIRE(ldx >= k && ldx % 8 == 0, "%s: ldx = %lld must be a multiple of 8 and at least K", op, static_cast<long long>(ldx));
-    FSO_REQUIRE(aligned16(x) && aligned16(codes), "%s: x and codes must be 16-byte aligned", op);
+    FSO_REQUIRE(aligned16(x) && aligned16(codes) && aligned16(scale) && aligned16(zero),
+        "%s: x, codes, scale and zero must be 16-byte aligned", op);
     return 0;
 }
 
@@ -785,27 +786,26 @@ int fso_int4_quantize(const void* w, void* codes, void* scale, void* zero, int64
     FSO_REQUIRE(vectors <= (1ll << 38), "fso_int4_quantize: N * K is too large for one launch");
     auto kernel = dtype == 0 ? int4_quantize_kernel<true> : int4_quantize_kernel<false>;
     kernel<<<blocks_for(vectors, 256), 256, 0, as_stream(stream)>>>(static_cast<uint4 const*>(w), static_cast<uint32_t*>(codes),
-        scale, static_cast<int>(scale_dtype), static_cast<uint8_t*>(zero), vectors, static_cast<int>(group / 8));
+        scale, static_cast<int>(scale_dtype), static_cast<uint8_t*>(zero), vectors, static_cast<int>(group / 8), (n + 1) / 2, int4_half_cols(n),
+        static_cast<int>(k / group));
     return launch_status("int4_quantize_kernel");
 }
 
 int fso_int4_linear(const void* x, int64_t ldx, const void* codes, const void* scale, const void* zero, const void* bias,
     void* y, int64_t m, int64_t n, int64_t k, int64_t group, int64_t dtype, int64_t scale_dtype, void* stream)
 {
-    int const rc = check_int4("fso_int4_linear", m, n, k, group, dtype, scale_dtype, x, ldx, codes, scale, y);
+    int const rc = check_int4("fso_int4_linear", m, n, k, group, dtype, scale_dtype, x, ldx, codes, scale, zero, y);
     if (rc != 0 || m == 0) return rc;
     Int4Params p{};
     p.x = x;
     p.ldx = ldx;
-    p.scale = scale;
     p.scale_type = static_cast<int>(scale_dtype);
-    p.zero = static_cast<uint8_t const*>(zero);
     p.bias = bias;
     p.out = y;
     p.m = static_cast<int>(m);
     p.k = static_cast<int>(k);
     p.out_cols = static_cast<int>(n);
-    return launch_int4(p, static_cast<uint8_t const*>(codes), group, dtype == 0, as_stream(stream));
+    return launch_int4(p, n, static_cast<uint8_t const*>(codes), scale, zero, group, dtype == 0, as_stream(stream));
 }
 
 int fso_int4_gated_linear(const void* x, int64_t ldx, const void* codes, const void* scale, const void* zero, void* h,
@@ -814,21 +814,19 @@ int fso_int4_gated_linear(const void* x, int64_t ldx, const void* codes, const v
     FSO_REQUIRE(inter > 0 && inter <= (1ll << 23), "fso_int4_gated_linear: INTER must be in [1, 2^23]");
     FSO_REQUIRE(activation >= 0 && activation <= 2,
         "fso_int4_gated_linear: activation must be 0 (silu), 1 (gelu) or 2 (gelu_tanh)");
-    int const rc = check_int4("fso_int4_gated_linear", m, 2 * inter, k, group, dtype, scale_dtype, x, ldx, codes, scale, h);
+    int const rc = check_int4("fso_int4_gated_linear", m, 2 * inter, k, group, dtype, scale_dtype, x, ldx, codes, scale, zero, h);
     if (rc != 0 || m == 0) return rc;
     Int4Params p{};
     p.x = x;
     p.ldx = ldx;
-    p.scale = scale;
     p.scale_type = static_cast<int>(scale_dtype);
-    p.zero = static_cast<uint8_t const*>(zero);
     p.out = h;
     p.m = static_cast<int>(m);
     p.k = static_cast<int>(k);
     p.out_cols = static_cast<int>(inter);
     p.gated = 1;
     p.act = static_cast<int>(activation);
-    return launch_int4(p, static_cast<uint8_t const*>(codes), group, dtype == 0, as_stream(stream));
+    return launch_int4(p, 2 * inter, static_cast<uint8_t const*>(codes), scale, zero, group, dtype == 0, as_stream(stream));
 }
 
 }  // extern "C"

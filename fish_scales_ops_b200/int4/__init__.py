@@ -29,40 +29,67 @@ _MAX_DIM = 1 << 24
 _MAX_ROWS = 65535 * 8
 
 
+def _by_halves(t: torch.Tensor) -> torch.Tensor:
+    """[N, groups] -> [groups, 2 * half], the layout the kernels read; columns between the halves are zero."""
+    n, first, half = t.shape[0], (t.shape[0] + 1) // 2, _ops.int4_half_cols(t.shape[0])
+    out = t.new_zeros((t.shape[1], 2 * half))
+    out[:, :first].copy_(t[:first].t())
+    out[:, half:half + n - first].copy_(t[first:].t())
+    return out
+
+
+def _rows_of(t: torch.Tensor, n: int) -> torch.Tensor:
+    """The inverse of :func:`_by_halves`."""
+    first, half = (n + 1) // 2, t.shape[1] // 2
+    return torch.cat((t[:, :first], t[:, half:half + n - first]), 1).t()
+
+
 @dataclasses.dataclass(frozen=True, eq=False, repr=False)
 class Int4Weight:
     """One 4-bit weight: ``codes`` uint8 ``[N, K/2]``, ``scale`` bf16, fp16 or fp32 ``[N, K/group_size]``, ``zero`` uint8
-    of the same shape or None (8 everywhere)."""
+    of the same shape or None (8 everywhere). The kernels read them transposed and by halves of the rows, as ``scale_t``
+    and ``zero_t`` ``[K/group_size, 2 * half]``: ``half`` is half of N rounded up to a multiple of 16, the first half of the
+    rows starts at column 0 and the second at column ``half``."""
 
     arch: int
     in_features: int
     out_features: int
     group_size: int
     codes: torch.Tensor
-    scale: torch.Tensor
-    zero: Optional[torch.Tensor]
+    scale_t: torch.Tensor
+    zero_t: Optional[torch.Tensor]
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return _rows_of(self.scale_t, self.out_features)
+
+    @property
+    def zero(self) -> Optional[torch.Tensor]:
+        return None if self.zero_t is None else _rows_of(self.zero_t, self.out_features)
 
     def __repr__(self) -> str:
         return (f"Int4Weight(arch=sm_{self.arch}, in_features={self.in_features}, out_features={self.out_features}, "
-                f"group_size={self.group_size}, scale={self.scale.dtype}, zero={'none' if self.zero is None else 'uint8'})")
+                f"group_size={self.group_size}, scale={self.scale_t.dtype}, zero={'none' if self.zero_t is None else 'uint8'})")
 
 
 def _check_weight(op: str, codes, scale, zero) -> None:
-    """The three tensors of a weight, by their metadata alone."""
+    """The three tensors of a weight as the kernels read them, by their metadata alone."""
     if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[0] < 1 or codes.shape[1] < 16:
         raise ValueError(f"{op}: codes must be a uint8 [N, K/2] tensor, two codes in a byte, got {codes.dtype} "
                          f"{tuple(codes.shape)}")
     n, k = int(codes.shape[0]), 2 * int(codes.shape[1])
-    if scale.dtype not in _SCALE_DTYPES or scale.dim() != 2 or scale.shape[0] != n or scale.shape[1] < 1:
-        raise ValueError(f"{op}: scale must be a bf16, fp16 or fp32 [{n}, K/group] tensor, got {scale.dtype} "
-                         f"{tuple(scale.shape)}")
-    group = k // int(scale.shape[1])
-    if group * int(scale.shape[1]) != k or group < 32 or group & (group - 1):
-        raise ValueError(f"{op}: {int(scale.shape[1])} scales for a row of K = {k}: the group size must be a power of two of "
-                         f"at least 32 that divides K")
+    cols = 2 * _ops.int4_half_cols(n)
+    if scale.dtype not in _SCALE_DTYPES or scale.dim() != 2 or scale.shape[1] != cols or scale.shape[0] < 1:
+        raise ValueError(f"{op}: scale must be bf16, fp16 or fp32 [K/group, {cols}] for {n} rows (the layout of "
+                         f"fso.int4.Int4Weight.scale_t), got {scale.dtype} {tuple(scale.shape)}")
+    groups = int(scale.shape[0])
+    group = k // groups
+    if group * groups != k or group < 32 or group & (group - 1):
+        raise ValueError(f"{op}: {groups} scales for a row of K = {k}: the group size must be a power of two of at least 32 "
+                         f"that divides K")
     if zero is not None and (zero.dtype != torch.uint8 or zero.shape != scale.shape):
-        raise ValueError(f"{op}: zero must be a uint8 {tuple(scale.shape)} tensor like scale, got {zero.dtype} "
-                         f"{tuple(zero.shape)}")
+        raise ValueError(f"{op}: zero must be uint8 and shaped like scale, got {zero.dtype} {tuple(zero.shape)} for "
+                         f"{tuple(scale.shape)}")
     if n > _MAX_DIM or k > _MAX_DIM:
         raise ValueError(f"{op}: a dimension of [{n}, {k}] is beyond 2^24")
     for name, t in (("codes", codes), ("scale", scale), ("zero", zero)):
@@ -169,18 +196,22 @@ def _int4_gated_linear_fake(x, codes, scale, zero, activation):
 def prepare_weight(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None) -> Int4Weight:
     """The handle of a weight that a checkpoint stores in 4 bits: ``codes`` uint8 ``[N, K/2]``, ``scale`` bf16, fp16 or
     fp32 ``[N, K/group]``, ``zero`` uint8 ``[N, K/group]`` with values 0..15 (None: 8 everywhere). The group size is a power
-    of two of at least 32. The tensors are kept as they are; one that is not contiguous or off a 16-byte boundary is
-    copied. The values of ``zero`` are not looked at (that would synchronize)."""
+    of two of at least 32. The codes are kept as they are (copied if they are not contiguous or off a 16-byte boundary),
+    scales and zero points are transposed. The values of ``zero`` are not looked at (that would synchronize)."""
     ctx = "fso.int4.prepare_weight"
     for name, t in (("codes", codes), ("scale", scale), ("zero", zero)):
         if not isinstance(t, torch.Tensor) and not (name == "zero" and t is None):
             raise ValueError(f"{ctx}: {name} must be a tensor, got {type(t).__name__}")
-    codes, scale = _aligned(codes.detach()), _aligned(scale.detach())
-    zero = None if zero is None else _aligned(zero.detach())
-    _check_weight(ctx, codes, scale, zero)
+    for name, t in (("scale", scale), ("zero", zero)):
+        if t is not None and (t.dim() != 2 or codes.dim() < 1 or t.shape[0] != codes.shape[0] or 0 in t.shape):
+            raise ValueError(f"{ctx}: {name} must be a [N, K/group] tensor for the codes' {codes.shape[0]} rows, got "
+                             f"{tuple(t.shape)}")
+    codes, scale_t = _aligned(codes.detach()), _by_halves(scale.detach())
+    zero_t = None if zero is None else _by_halves(zero.detach())
+    _check_weight(ctx, codes, scale_t, zero_t)
     _need_arch(ctx)
     k = 2 * int(codes.shape[1])
-    return _complete(Int4Weight(device_arch(), k, int(codes.shape[0]), k // int(scale.shape[1]), codes, scale, zero))
+    return _complete(Int4Weight(device_arch(), k, int(codes.shape[0]), k // int(scale_t.shape[0]), codes, scale_t, zero_t))
 
 
 def quantize_weight(w: torch.Tensor, *, group_size: int = 128, zero_point: bool = False,
@@ -224,12 +255,12 @@ def linear(x: torch.Tensor, weight: Int4Weight, *, bias: Optional[torch.Tensor] 
     of the same shape."""
     x2 = _flatten(x, weight, "fso.int4.linear")
     if torch.compiler.is_compiling():
-        y = torch.ops.fish_scales_ops.int4_linear(x2, weight.codes, weight.scale, weight.zero, bias)
+        y = torch.ops.fish_scales_ops.int4_linear(x2, weight.codes, weight.scale_t, weight.zero_t, bias)
     else:
         _check_x("fso.int4.linear", x2, weight.codes)
         if bias is not None:
             _check_bias("fso.int4.linear", bias, x2, weight.out_features)
-        y = _ops.int4_linear(x2, weight.codes, weight.scale, weight.zero, bias)
+        y = _ops.int4_linear(x2, weight.codes, weight.scale_t, weight.zero_t, bias)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.out_features)
 
 
@@ -239,9 +270,9 @@ def gated_linear(x: torch.Tensor, gate_up: Int4Weight, *, activation: str = "sil
     ``"silu"``, ``"gelu"`` (erf) or ``"gelu_tanh"``. Otherwise as :func:`linear`."""
     x2 = _flatten(x, gate_up, "fso.int4.gated_linear")
     if torch.compiler.is_compiling():
-        h = torch.ops.fish_scales_ops.int4_gated_linear(x2, gate_up.codes, gate_up.scale, gate_up.zero, activation)
+        h = torch.ops.fish_scales_ops.int4_gated_linear(x2, gate_up.codes, gate_up.scale_t, gate_up.zero_t, activation)
     else:
         _check_gate("fso.int4.gated_linear", gate_up.codes, activation)
         _check_x("fso.int4.gated_linear", x2, gate_up.codes)
-        h = _ops.int4_gated_linear(x2, gate_up.codes, gate_up.scale, gate_up.zero, _ops.GATE_ACTIVATIONS[activation])
+        h = _ops.int4_gated_linear(x2, gate_up.codes, gate_up.scale_t, gate_up.zero_t, _ops.GATE_ACTIVATIONS[activation])
     return h if x.dim() == 2 else h.reshape(*x.shape[:-1], gate_up.out_features // 2)

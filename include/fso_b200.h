@@ -289,9 +289,12 @@ int fso_gated_linear_backward(const void* dh, int64_t ldh, const void* x, int64_
 /* ---- Linear layers over 4-bit weights with group scales ------------------------------------------------------------
  *
  * W[n, k] = scale[n, k / group] * (code[n, k] - zero[n, k / group]); codes two in a byte, even k in the lower four bits,
- * rows of K / 2 bytes; scale bf16 (0), fp16 (1) or fp32 (2) [N, K / group]; zero uint8 of the same shape, or NULL for 8.
- * group is a power of two of at least 32 that divides K. x 16 bit [M, ldx] (dtype 0 = bf16, 1 = fp16), ldx % 8 == 0; codes
- * and x 16-byte aligned. y[m] = x[m] W^T (+ bias), h[m] = act(x[m] G^T) * (x[m] U^T) with G, U the first and the last
+ * rows of K / 2 bytes. scale, bf16 (0), fp16 (1) or fp32 (2), lies transposed and by halves of the rows, so that the
+ * scales of neighbouring rows are read together from 16-byte boundaries: [K / group, 2 * half] with half = (N + 1) / 2 rounded
+ * up to a multiple of 16; row n of the first (N + 1) / 2 rows is column n, a later row n is column half + n - (N + 1) / 2; the
+ * columns between are not used. zero, uint8, lies the same way, or NULL for 8.
+ * group is a power of two of at least 32 that divides K. x 16 bit [M, ldx] (dtype 0 = bf16, 1 = fp16), ldx % 8 == 0; x, codes,
+ * scale and zero 16-byte aligned. y[m] = x[m] W^T (+ bias), h[m] = act(x[m] G^T) * (x[m] U^T) with G, U the first and the last
  * INTER rows of W; both contiguous. The whole number code - zero enters its product exactly, sums and scales are
  * fp32, the result is rounded once. Built for the few rows of a decode step. No counterpart in the reference, which
  * serves 8-bit weights (python/fish_scales_ops/dense/__init__.py:121-140). */

@@ -47,7 +47,7 @@ def test_prepare_weight_refuses(fso, codes, scale, zero, text):
 
 
 def test_linear_refuses(fso):
-    handle = fso.int4.Int4Weight(100, 128, 4, 64, _z(4, 64, dtype=torch.uint8), _z(4, 2), None)
+    handle = fso.int4.Int4Weight(100, 128, 4, 64, _z(4, 64, dtype=torch.uint8), _z(2, 32), None)
     with pytest.raises(TypeError, match="Int4Weight"):
         fso.int4.linear(_z(2, 128), _z(4, 128))
     for call in (fso.int4.linear, fso.int4.gated_linear):
