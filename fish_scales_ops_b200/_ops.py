@@ -350,46 +350,63 @@ def rows_in_place(x: torch.Tensor):
     return x.clone(memory_format=torch.contiguous_format), k
 
 
+_GATED_WS = {}
+
+
+def _gated_ws_bytes(query: str, t: int, k: int, inter: int, dev: int) -> int:
+    """Workspace of a gated projection's forward or backward pass: a function of the sizes and the device's SM count,
+    asked once for each."""
+    key = (query, t, k, inter, dev)
+    if key not in _GATED_WS:
+        if len(_GATED_WS) > 4096:      # prompts of ever new lengths
+            _GATED_WS.clear()
+        need = ctypes.c_int64(0)
+        check(getattr(lib(), query)(t, k, inter, ctypes.byref(need)), query)
+        _GATED_WS[key] = need.value
+    return _GATED_WS[key]
+
+
 def gated_linear(x, gate_up, activation: int, save: bool):
-    """x [T, K], gate_up [2I, K] -> (h [T, I], saved upper 16 bits, saved lower 8 bits); the saved arrays are empty
+    """x [T, K], gate_up [2I, K] -> (h [T, I], saved upper 16 bits, saved lower 8 bits); the saved arrays are None
     without ``save``."""
-    t, k = int(x.shape[0]), int(x.shape[1])
-    inter = int(gate_up.shape[0]) // 2
-    with on_device(x.device):
-        h = torch.empty((t, inter), dtype=x.dtype, device=x.device)
-        cols = 2 * _align(inter, 16) if save else 0
-        hi = torch.empty((t, cols), dtype=torch.int16, device=x.device)
-        lo = torch.empty((t, cols), dtype=torch.uint8, device=x.device)
-        if t > 0:
-            x, ldx = rows_in_place(x)
-            need = ctypes.c_int64(0)
-            check(lib().fso_gated_linear_ws_bytes(t, k, inter, ctypes.byref(need)), "fso_gated_linear_ws_bytes")
-            ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device) if need.value else None
-            check(lib().fso_gated_linear(ptr(x), ldx, ptr(gate_up), ptr(h), ptr(hi) if save else None,
-                                         ptr(lo) if save else None, t, k, inter, DTYPES_16[x.dtype], activation, ptr(ws),
-                                         need.value, stream_ptr()), "fso_gated_linear")
+    t, k = x.shape
+    inter = gate_up.shape[0] // 2
+    h = x.new_empty((t, inter))
+    hi = lo = None
+    if save:
+        cols = 2 * _align(inter, 16)
+        hi, lo = x.new_empty((t, cols), dtype=torch.int16), x.new_empty((t, cols), dtype=torch.uint8)
+    if t > 0:
+        x, ldx = rows_in_place(x)
+        with on_device(x.device):
+            need = _gated_ws_bytes("fso_gated_linear_ws_bytes", t, k, inter, x.get_device())
+            ws = x.new_empty((need,), dtype=torch.uint8) if need else None
+            rc = call_on(x, lib().fso_gated_linear, x.data_ptr(), ldx, gate_up.data_ptr(), h.data_ptr(),
+                         hi.data_ptr() if save else None, lo.data_ptr() if save else None, t, k, inter, DTYPES_16[x.dtype],
+                         activation, None if ws is None else ws.data_ptr(), need)
+        if rc != 0:
+            check(rc, "fso_gated_linear")
     return h, hi, lo
 
 
 def gated_linear_backward(dh, x, gate_up, hi, lo, activation: int, need_x: bool, need_w: bool):
     """(dx [T, K] or empty, dgate_up [2I, K] or empty) for dh [T, I]."""
-    t, k = int(x.shape[0]), int(x.shape[1])
-    inter = int(gate_up.shape[0]) // 2
-    with on_device(x.device):
-        dx = torch.empty((t if need_x else 0, k), dtype=x.dtype, device=x.device)
-        dw = (torch.empty if t > 0 else torch.zeros)((2 * inter if need_w else 0, k), dtype=x.dtype, device=x.device)
-        if t > 0 and (need_x or need_w):
-            x, ldx = rows_in_place(x)
-            if (inter > 1 and dh.stride(1) != 1) or (t > 1 and dh.stride(0) < inter):
-                dh = dh.contiguous()
-            need = ctypes.c_int64(0)
-            check(lib().fso_gated_linear_backward_ws_bytes(t, k, inter, ctypes.byref(need)),
-                  "fso_gated_linear_backward_ws_bytes")
-            ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device)
-            check(lib().fso_gated_linear_backward(ptr(dh), dh.stride(0) if t > 1 else inter, ptr(x), ldx, ptr(gate_up),
-                                                  ptr(hi), ptr(lo), ptr(dx) if need_x else None,
-                                                  ptr(dw) if need_w else None, t, k, inter, DTYPES_16[x.dtype], activation,
-                                                  ptr(ws), need.value, stream_ptr()), "fso_gated_linear_backward")
+    t, k = x.shape
+    inter = gate_up.shape[0] // 2
+    dx = x.new_empty((t if need_x else 0, k))
+    dw = (x.new_empty if t > 0 else x.new_zeros)((2 * inter if need_w else 0, k))
+    if t > 0 and (need_x or need_w):
+        x, ldx = rows_in_place(x)
+        if (inter > 1 and dh.stride(1) != 1) or (t > 1 and dh.stride(0) < inter):
+            dh = dh.contiguous()
+        with on_device(x.device):
+            need = _gated_ws_bytes("fso_gated_linear_backward_ws_bytes", t, k, inter, x.get_device())
+            ws = x.new_empty((need,), dtype=torch.uint8)
+            rc = call_on(x, lib().fso_gated_linear_backward, dh.data_ptr(), dh.stride(0) if t > 1 else inter, x.data_ptr(), ldx,
+                         gate_up.data_ptr(), hi.data_ptr(), lo.data_ptr(), dx.data_ptr() if need_x else None,
+                         dw.data_ptr() if need_w else None, t, k, inter, DTYPES_16[x.dtype], activation, ws.data_ptr(), need)
+        if rc != 0:
+            check(rc, "fso_gated_linear_backward")
     return dx, dw
 
 

@@ -495,6 +495,215 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
     }
 }
 
+// ------------------------------------------------------------------------------------------------ few rows
+//
+// The forward pass for at most 128 rows of x, where the weight bytes are the cost: 64 rows of G and the same 64 rows of U on
+// MMA-M, the rows of x on MMA-N, one tile for each CTA and two CTAs to an SM, so that more than a hundred kilobytes of
+// an SM's weights are on their way at any time. Where the tiles leave SMs without work the CTAs of a cluster split the
+// contraction, and each adds up its part of the outputs over distributed shared memory, in a fixed order.
+// Nothing is read before the preceding kernel has finished: unlike a prepared weight, gate_up may be its output.
+template <int BN>
+struct GatedRowsCfg {
+    static constexpr int kThreads = 192;       // TMA, MMA, four warps for the accumulators
+    static constexpr int kABytes = 128 * 128;
+    static constexpr int kBBytes = BN * 128;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kStages = (110 * 1024) / kStageBytes;
+    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+    static constexpr int kRedStride = 132;     // floats between the rows of x in the sums of a slice
+    static constexpr int kTmemCols = BN < 32 ? 32 : BN;
+    static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
+    static_assert(BN * kRedStride * 4 <= kStages * kStageBytes, "the sums fit the stages");
+};
+
+struct GatedRowsParams {
+    int t, inter, act;
+    int kb_total, kb_per_split, splits;
+    void* out;
+    uint16_t* save_hi;
+    uint8_t* save_lo;
+    int64_t half_cols;
+};
+
+__device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
+template <int BN, bool kBf16>
+__global__ void __launch_bounds__(GatedRowsCfg<BN>::kThreads, 2)
+gated_rows_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ CUtensorMap tm_u,
+    const __grid_constant__ CUtensorMap tm_x, const GatedRowsParams p)
+{
+    using C = GatedRowsCfg<BN>;
+    constexpr int S = C::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint32_t const raw = smem_u32(smem_raw);
+    uint32_t const base = (raw + 1023u) & ~1023u;
+    uint8_t* const gbase = smem_raw + (base - raw);
+    uint32_t const sA = base, sB = base + S * C::kABytes;
+    uint32_t const bars = base + S * C::kStageBytes;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
+    uint32_t const done_bar = bars + 16u * S;
+    uint32_t const misc = S * C::kStageBytes + 16 * S + 8;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + misc);
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(gbase + misc + 4);
+
+    int const warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+    int const lane = threadIdx.x & 31;
+    int const tile = blockIdx.x / p.splits;
+    int const rank = blockIdx.x - tile * p.splits;
+    int const kb0 = rank * p.kb_per_split, kb1 = min(p.kb_total, kb0 + p.kb_per_split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(done_bar, 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t const tmem_base = *tmem_slot;
+    griddep_launch_dependents();
+    griddep_wait();
+
+    if (warp == 0) {
+        if (elect_one()) {
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!wait_or_abort(empty_bar(stage), phase ^ 1u, abort_flag)) {
+                    record_abort(FSO_DEV_WAIT_PRODUCER, abort_flag);
+                    break;
+                }
+                uint32_t const fb = full_bar(stage);
+                mbar_expect_tx(fb, C::kStageBytes);
+                tma_load_2d(sA + stage * C::kABytes, &tm_g, fb, kb * 64, tile * 64);
+                tma_load_2d(sA + stage * C::kABytes + 8192, &tm_u, fb, kb * 64, tile * 64);
+                tma_load_2d(sB + stage * C::kBBytes, &tm_x, fb, kb * 64, 0);
+                if (++stage == S) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (elect_one()) {
+            constexpr uint32_t idesc = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | ((BN >> 3) << 17) | ((128u >> 4) << 24);
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!wait_or_abort(full_bar(stage), phase, abort_flag)) {
+                    record_abort(FSO_DEV_WAIT_MMA_FULL, abort_flag);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                uint64_t const adesc = make_desc_sw128(sA + stage * C::kABytes), bdesc = make_desc_sw128(sB + stage * C::kBBytes);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc_mma_f16(tmem_base, adesc + 2u * k, bdesc + 2u * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                tc_commit(empty_bar(stage));
+                if (++stage == S) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (ok) tc_commit(done_bar);
+        }
+        __syncwarp();
+    } else {
+        // the accumulators of a slice to shared memory: every stage has been read by the time they are complete
+        if (wait_or_abort(done_bar, 0, abort_flag)) {
+            __syncwarp();
+            tc_fence_after();
+            int const quarter = warp & 3;
+            float* const red = reinterpret_cast<float*>(gbase) + quarter * 32 + lane;
+            uint32_t const t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 16) {
+                if (c >= p.t) break;
+                uint32_t r[16];
+                tmem_ld_32x16(t_row + c, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) red[(c + j) * C::kRedStride] = __uint_as_float(r[j]);
+            }
+            tc_fence_before();
+        } else if (lane == 0) {
+            record_abort(FSO_DEV_WAIT_EPILOGUE, abort_flag);
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    bool const failed = *abort_flag != 0;
+    if (failed) {
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);      // copies in flight land before the memory is given up
+        __syncthreads();
+    }
+    if (p.splits > 1) cluster_sync_all();
+    if (!failed) {
+        float const* const red = reinterpret_cast<float const*>(gbase);
+        uint32_t const red_addr = smem_u32(red);
+        for (int i = rank * C::kThreads + static_cast<int>(threadIdx.x); i < p.t * 64; i += C::kThreads * p.splits) {
+            int const row = i >> 6, in_tile = i & 63;
+            int const col = tile * 64 + in_tile;
+            if (col >= p.inter) continue;
+            int const at = row * C::kRedStride + in_tile;
+            float g = 0.f, u = 0.f;
+            if (p.splits == 1) {
+                g = red[at];
+                u = red[at + 64];
+            } else {
+                for (int r = 0; r < p.splits; ++r) {
+                    uint32_t const peer = map_to_cta(red_addr + 4u * at, r);
+                    g += ld_cluster_f32(peer);
+                    u += ld_cluster_f32(peer + 256u);
+                }
+            }
+            if (p.save_hi != nullptr) {
+                int64_t const to = static_cast<int64_t>(row) * 2 * p.half_cols + col;
+                uint32_t const gb = to_24(g), ub = to_24(u);
+                p.save_hi[to] = static_cast<uint16_t>(gb >> 8);
+                p.save_lo[to] = static_cast<uint8_t>(gb);
+                p.save_hi[to + p.half_cols] = static_cast<uint16_t>(ub >> 8);
+                p.save_lo[to + p.half_cols] = static_cast<uint8_t>(ub);
+            }
+            store16<kBf16>(p.out, static_cast<int64_t>(row) * p.inter + col, gate_value(g, p.act) * u);
+        }
+    }
+    __syncwarp();
+    if (p.splits > 1) cluster_sync_all();      // no CTA leaves while another may still read its sums
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::kTmemCols);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ split sums
 
 // out = the sum of the slices of the contraction, in their order, rounded once. Columns are multiples of 8.
@@ -625,6 +834,8 @@ inline int make_map16(CUtensorMap* map, const void* base, int64_t rows, int64_t 
 
 inline int64_t gated_half_cols(int64_t inter) { return (inter + 15) / 16 * 16; }
 
+constexpr int kGatedRowsMax = 128;      // rows of x up to which the few-rows kernel runs the forward pass
+
 // Tiles and slices of one of the three products. Pure host arithmetic.
 struct Gated16Plan {
     int tiles_m, tiles_half, tiles_n, kb, kb_half, splits, kb_per_split;
@@ -637,6 +848,7 @@ inline Gated16Plan plan_gated16(int mode, int64_t t, int64_t k, int64_t inter, i
     auto tiles = [](int64_t n, int64_t w) { return static_cast<int>((n + w - 1) / w); };
     int64_t rows = t, ws_cols = k;
     if (mode == G16_GATED) {
+        if (t <= kGatedRowsMax) return p;      // no workspace
         p.tiles_m = tiles(t, 256);
         p.tiles_n = tiles(inter, 128);
         p.kb = tiles(k, 64);
@@ -688,10 +900,67 @@ inline void fill_gated16(Gated16Params& p, Gated16Plan const& pl)
 
 inline unsigned blocks_for(int64_t threads, int per_block) { return static_cast<unsigned>((threads + per_block - 1) / per_block); }
 
+// Slices of the contraction for `tiles` CTAs' worth of rows: as many as all SMs need to have work (two CTAs fit), at most
+// eight (the portable cluster size), at least four 64-wide blocks in each and none empty.
+inline void gated_rows_slices(int64_t tiles, int kb, int sms, GatedRowsParams& p)
+{
+    int s = 1;
+    while (s < 8 && tiles * s * 2 <= 3 * sms && (s + 1) * 4 <= kb) ++s;
+    p.kb_total = kb;
+    p.kb_per_split = (kb + s - 1) / s;
+    p.splits = (kb + p.kb_per_split - 1) / p.kb_per_split;
+}
+
+template <int BN, bool kBf16>
+inline int launch_gated_rows(const void* x, int64_t ldx, const void* gate_up, int64_t k, GatedRowsParams p, cudaStream_t stream)
+{
+    using C = GatedRowsCfg<BN>;
+    static std::atomic<uint64_t> done{0};
+    auto kernel = gated_rows_kernel<BN, kBf16>;
+    int rc = ensure_smem_attr(kernel, C::kSmemBytes, done);
+    if (rc != 0) return rc;
+    uint16_t const* const w = static_cast<uint16_t const*>(gate_up);
+    CUtensorMap mg, mu, mx;
+    rc = make_map16(&mg, w, p.inter, k, k, 64);
+    if (rc == 0) rc = make_map16(&mu, w + p.inter * k, p.inter, k, k, 64);
+    if (rc == 0) rc = make_map16(&mx, x, p.t, k, ldx, BN);
+    if (rc != 0) return rc;
+    int const tiles = (p.inter + 63) / 64;
+    gated_rows_slices(tiles, static_cast<int>((k + 63) / 64), sm_count(), p);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.splits), 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(p.splits);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1 + pdl_attribute(&attr[1]);
+    FSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, mg, mu, mx, p));
+    return launch_status("gated_rows_kernel");
+}
+
 template <bool kBf16>
 inline int gated_forward(const void* x, int64_t ldx, const void* gate_up, void* h, void* save_hi, void* save_lo, int64_t t,
     int64_t k, int64_t inter, int act, void* ws, cudaStream_t stream)
 {
+    if (t <= kGatedRowsMax) {
+        GatedRowsParams r{};
+        r.t = static_cast<int>(t);
+        r.inter = static_cast<int>(inter);
+        r.act = act;
+        r.out = h;
+        r.save_hi = static_cast<uint16_t*>(save_hi);
+        r.save_lo = static_cast<uint8_t*>(save_lo);
+        r.half_cols = gated_half_cols(inter);
+        return t <= 16 ? launch_gated_rows<16, kBf16>(x, ldx, gate_up, k, r, stream)
+            : t <= 32  ? launch_gated_rows<32, kBf16>(x, ldx, gate_up, k, r, stream)
+            : t <= 64  ? launch_gated_rows<64, kBf16>(x, ldx, gate_up, k, r, stream)
+                       : launch_gated_rows<128, kBf16>(x, ldx, gate_up, k, r, stream);
+    }
     int const sms = sm_count();
     Gated16Plan const pl = plan_gated16(G16_GATED, t, k, inter, sms);
     CUtensorMap m[4];

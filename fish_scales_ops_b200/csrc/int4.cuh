@@ -74,13 +74,6 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t saddr, uint32_t (&r)[4])
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(saddr) : "memory");
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
-{
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
-    return v;
-}
-
 template <int NT>
 struct Int4Cfg {
     static constexpr int kRT = 2;                // 16-row tiles of a warp

@@ -22,48 +22,53 @@ _MAX_DIM = 1 << 24
 
 
 def _check(op: str, x, gate_up, activation) -> None:
+    """``op``: the name in a refusal, which begins with the device's."""
     if activation not in _ops.GATE_ACTIVATIONS:
-        raise ValueError(f"{op}: unknown activation {activation!r}; the activations are {', '.join(ACTIVATIONS)}")
+        _refuse(op, f"unknown activation {activation!r}; the activations are {', '.join(ACTIVATIONS)}")
     if x.dim() != 2 or gate_up.dim() != 2 or x.shape[1] != gate_up.shape[1]:
-        raise ValueError(f"{op}: x must be [..., K] and gate_up [2*INTER, K] with the same K, got {tuple(x.shape)} and "
-                         f"{tuple(gate_up.shape)}")
+        _refuse(op, f"x must be [..., K] and gate_up [2*INTER, K] with the same K, got {tuple(x.shape)} and "
+                    f"{tuple(gate_up.shape)}")
     if x.dtype not in _ops.DTYPES_16 or gate_up.dtype != x.dtype:
-        raise ValueError(f"{op}: x and gate_up must both be bf16 or both fp16, got {x.dtype} and {gate_up.dtype}")
-    if not x.is_cuda or gate_up.device != x.device:
-        raise ValueError(f"{op}: x and gate_up must be on one CUDA device, got {x.device} and {gate_up.device}")
-    rows, k = int(gate_up.shape[0]), int(gate_up.shape[1])
+        _refuse(op, f"x and gate_up must both be bf16 or both fp16, got {x.dtype} and {gate_up.dtype}")
+    if not x.is_cuda or gate_up.get_device() != x.get_device():
+        _refuse(op, f"x and gate_up must be on one CUDA device, got {x.device} and {gate_up.device}")
+    rows, k = gate_up.shape
     if rows < 2 or rows % 2 != 0 or k < 8 or k % 8 != 0:
-        raise ValueError(f"{op}: gate_up must have an even number of rows and K a positive multiple of 8, got "
-                         f"{tuple(gate_up.shape)}")
-    if max(rows // 2, k, int(x.shape[0])) > _MAX_DIM:
-        raise ValueError(f"{op}: a dimension of {tuple(x.shape)} or {tuple(gate_up.shape)} is beyond 2^24")
+        _refuse(op, f"gate_up must have an even number of rows and K a positive multiple of 8, got {tuple(gate_up.shape)}")
+    if rows // 2 > _MAX_DIM or k > _MAX_DIM or x.shape[0] > _MAX_DIM:
+        _refuse(op, f"a dimension of {tuple(x.shape)} or {tuple(gate_up.shape)} is beyond 2^24")
     if not gate_up.is_contiguous() or gate_up.data_ptr() % 16 != 0:
-        raise ValueError(f"{op}: gate_up must be contiguous and start on a 16-byte boundary (it is read in place with "
-                         f"TMA), got strides {tuple(gate_up.stride())}")
+        _refuse(op, f"gate_up must be contiguous and start on a 16-byte boundary (it is read in place with TMA), got strides "
+                    f"{tuple(gate_up.stride())}")
     if device_arch() // 10 != SERVED_MAJOR:
-        raise NotImplementedError(f"{op}: this build serves sm_100-family devices")
+        raise NotImplementedError(f"{op} ({arch_label(device_arch())}): this build serves sm_100-family devices")
+
+
+def _refuse(op: str, why: str):
+    raise ValueError(f"{op} ({arch_label(device_arch())}): {why}")
 
 
 # ------------------------------------------------------------------------------------------------ custom ops
 
 def _gated_linear_body(x, gate_up, activation, save):
-    op = f"fish_scales_ops::gated_linear ({arch_label(device_arch())})"
-    _check(op, x, gate_up, activation)
-    return _ops.gated_linear(x, gate_up, _ops.GATE_ACTIVATIONS[activation], save)
+    _check("fish_scales_ops::gated_linear", x, gate_up, activation)
+    h, hi, lo = _ops.gated_linear(x, gate_up, _ops.GATE_ACTIVATIONS[activation], save)
+    if not save:
+        hi, lo = (x.new_empty((x.shape[0], 0), dtype=d) for d in (torch.int16, torch.uint8))
+    return h, hi, lo
 
 
 def _gated_linear_backward_body(dh, x, gate_up, saved_hi, saved_lo, activation, need_x, need_w):
-    op = f"fish_scales_ops::gated_linear_backward ({arch_label(device_arch())})"
+    op = "fish_scales_ops::gated_linear_backward"
     _check(op, x, gate_up, activation)
     t, inter = int(x.shape[0]), int(gate_up.shape[0]) // 2
     cols = 2 * _ops._align(inter, 16)
     if tuple(dh.shape) != (t, inter) or dh.dtype != x.dtype or dh.device != x.device:
-        raise ValueError(f"{op}: dh must be {x.dtype} [{t}, {inter}] on {x.device}, got {dh.dtype} {tuple(dh.shape)} on "
-                         f"{dh.device}")
+        _refuse(op, f"dh must be {x.dtype} [{t}, {inter}] on {x.device}, got {dh.dtype} {tuple(dh.shape)} on {dh.device}")
     for s, dtype in ((saved_hi, torch.int16), (saved_lo, torch.uint8)):
         if tuple(s.shape) != (t, cols) or s.dtype != dtype or s.device != x.device or not s.is_contiguous():
-            raise ValueError(f"{op}: the saved arrays must be the int16 and the uint8 [{t}, {cols}] that "
-                             f"fish_scales_ops::gated_linear returned with save, got {s.dtype} {tuple(s.shape)}")
+            _refuse(op, f"the saved arrays must be the int16 and the uint8 [{t}, {cols}] that fish_scales_ops::gated_linear "
+                        f"returned with save, got {s.dtype} {tuple(s.shape)}")
     return _ops.gated_linear_backward(dh, x, gate_up, saved_hi, saved_lo, _ops.GATE_ACTIVATIONS[activation], need_x, need_w)
 
 
@@ -121,11 +126,13 @@ _gated_linear_op.register_autograd(_op_backward, setup_context=_setup_context)
 
 
 class _GatedLinear(torch.autograd.Function):
-    """The eager form: the bodies of the two custom ops, without the dispatcher's round trip."""
+    """The eager form: the kernels behind the two custom ops, without the dispatcher's round trip and with the checks made
+    once."""
 
     @staticmethod
     def forward(ctx, x, gate_up, activation):
-        h, hi, lo = _gated_linear_body(x, gate_up, activation, True)
+        _check("fso.ffn.gated_linear", x, gate_up, activation)
+        h, hi, lo = _ops.gated_linear(x, gate_up, _ops.GATE_ACTIVATIONS[activation], True)
         ctx.save_for_backward(x, gate_up, hi, lo)
         ctx.activation = activation
         return h
@@ -133,7 +140,11 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        return (*_gradients(_gated_linear_backward_body, ctx, dh), None)
+        return (*_gradients(_eager_backward, ctx, dh), None)
+
+
+def _eager_backward(dh, x, gate_up, hi, lo, activation, need_x, need_w):
+    return _ops.gated_linear_backward(dh, x, gate_up, hi, lo, _ops.GATE_ACTIVATIONS[activation], need_x, need_w)
 
 
 # ------------------------------------------------------------------------------------------------ public functions
@@ -160,5 +171,6 @@ def gated_linear(x: torch.Tensor, gate_up: torch.Tensor, *, activation: str = "s
     elif grad:
         h = _GatedLinear.apply(x2, gate_up, activation)
     else:
-        h = _gated_linear_body(x2, gate_up, activation, False)[0]
+        _check("fso.ffn.gated_linear", x2, gate_up, activation)
+        h = _ops.gated_linear(x2, gate_up, _ops.GATE_ACTIVATIONS[activation], False)[0]
     return h if x.dim() == 2 else h.reshape(*lead, h.shape[1])
