@@ -4,10 +4,11 @@
 //   dx         dg G + du U                     A = [dg | du], B = [G ; U], the two halves of the contraction in turn
 //   dG, dU     dg^T x, du^T x                  A = dg^T or du^T, B = x
 //
-// with dg = dh * u * act'(g), du = dh * act(g) (gated_slopes_kernel). All three are one kernel, a 256 x 256 tile for
-// each pair of CTAs (tcgen05.mma kind::f16, cta_group::2, fp32 accumulators in tensor memory), fed by TMA. The operand
-// whose contraction runs down its columns (G, U in dx; all operands of dG, dU) is staged as it lies in memory and
-// read by the tensor cores "M/N-major": nothing is transposed in memory.
+// with dg = dh * u * act'(g), du = dh * act(g) (gated_slopes_kernel). All are a 256 x 256 tile for each pair of CTAs
+// (tcgen05.mma kind::f16, cta_group::2, fp32 accumulators in tensor memory), fed by TMA. The operand whose contraction
+// runs down its columns (G, U in dx; all operands of dG, dU) is staged as it lies in memory and read by the tensor
+// cores "M/N-major": nothing is transposed in memory. The two products of the backward pass share one launch, so that the
+// tiles of one fill the rounds that the other leaves open.
 //
 // What bounds it: the tensor pipe for T from a few hundred on (an MMA of 256 x 256 x 16 takes 128 cycles), the weight
 // bytes below that.
@@ -19,7 +20,7 @@
 
 namespace fso {
 
-enum : int { G16_GATED = 0, G16_DX = 1, G16_DW = 2 };
+enum : int { G16_FORWARD = 0, G16_BACKWARD = 1 };
 enum : int { FSO_ACT_SILU = 0, FSO_ACT_GELU = 1, FSO_ACT_GELU_TANH = 2 };
 
 struct Gated16Cfg {
@@ -33,36 +34,42 @@ struct Gated16Cfg {
     static_assert(kSmemBytes <= 227 * 1024 && kSmemBytes > 116 * 1024, "one CTA per SM");
 };
 
-struct Gated16Params {
-    int rows;            // valid rows of the output (G16_DW: of one half)
+// One product: its tiles, the slices of its contraction and its output.
+struct Gated16Product {
+    int rows;            // valid rows of the output (dW: of one half)
     int cols;            // valid columns of the output
-    int tiles_m;         // 256-row tiles (G16_DW: of both halves)
-    int tiles_half;      // G16_DW: 256-row tiles of one half
+    int tiles_m;         // 256-row tiles (dW: of both halves)
     int tiles_n;
     int group_m;         // raster: row tiles walked together before the columns advance
     int kb_total;        // 64-wide blocks of the contraction
-    int kb_half;         // G16_DX: blocks of the first half
+    int kb_half;         // dx: blocks of the first half; dW: 256-row tiles of one half
     int splits;
     int kb_per_split;
-    int act;
     int vec;             // rows of `out` start on 16-byte boundaries
     void* out;           // 16 bit [rows, ldo]
     int64_t ldo;
-    int64_t out_half;    // G16_DW: elements from the first half's output to the second's
-    uint16_t* save_hi;   // G16_GATED: upper 16 of the 24 bits kept of g and u, [rows, 2 * half_cols], or nullptr
-    uint8_t* save_lo;    // G16_GATED: lower 8 bits
-    int64_t half_cols;   // columns from g to u in the saved arrays and in split sums
-    float* ws;           // splits > 1: fp32 sums [splits, rows, ws_cols] (G16_DW: [splits, 2, rows, ws_cols])
+    int64_t out_half;    // dW: elements from the first half's output to the second's
+    float* ws;           // splits > 1: fp32 sums [splits, rows, ws_cols] (dW: [splits, 2, rows, ws_cols])
     int64_t ws_cols;
+};
+
+struct Gated16Params {
+    Gated16Product first, second;      // forward: first alone; backward: in either order, tiles_m = 0 where one is not wanted
+    int first_is_dw;
+    int act;
+    uint16_t* save_hi;   // forward: upper 16 of the 24 bits kept of g and u, [rows, 2 * half_cols], or nullptr
+    uint8_t* save_lo;    // forward: lower 8 bits
+    int64_t half_cols;   // columns from g to u in the saved arrays and in split sums
 };
 
 // ------------------------------------------------------------------------------------------------ activations
 //
 // a = act(g) and s = act'(g), from act(g) = g P(g): P is the logistic function of g (silu), the normal distribution
 // function (gelu), or the logistic function of 2 z, z = sqrt(2/pi) (g + 0.044715 g^3), which is 0.5 (1 + tanh z).
-// The logistic function goes through the exponential and one division, so its relative error stays below 1e-5 in both
-// tails; 16-bit outputs cannot see it.
-__device__ __forceinline__ float logistic(float v) { return 1.f / (1.f + __expf(-v)); }
+// The logistic function goes through the exponential and an approximate division (2 ulp; zero past 2^126, where the
+// function is below 1e-37), so its relative error stays below 1e-5 in both tails; 16-bit outputs cannot see it. 1 - P
+// in the slopes loses digits only where it is added to P next to 1.
+__device__ __forceinline__ float logistic(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 
 constexpr float kGeluC = 0.79788456080286535588f;      // sqrt(2 / pi)
 constexpr float kGeluCubic = 0.044715f;
@@ -79,14 +86,14 @@ __device__ __forceinline__ void gate_value_slope(float g, int act, float& a, flo
     float p, dp;      // dp = g P'(g)
     if (act == FSO_ACT_SILU) {
         p = logistic(g);
-        dp = g * p * logistic(-g);
+        dp = g * p * (1.f - p);
     } else if (act == FSO_ACT_GELU) {
         p = normcdff(g);
         dp = g * 0.39894228040143267794f * __expf(-0.5f * g * g);
     } else {
         float const z2 = 2.f * kGeluC * (g + kGeluCubic * g * g * g);
         p = logistic(z2);
-        dp = g * p * logistic(-z2) * 2.f * kGeluC * (1.f + 3.f * kGeluCubic * g * g);
+        dp = g * p * (1.f - p) * 2.f * kGeluC * (1.f + 3.f * kGeluCubic * g * g);
     }
     a = g * p;
     s = p + dp;
@@ -221,14 +228,15 @@ __device__ __forceinline__ void tc_mma_f16_pair(uint32_t d_tmem, uint64_t adesc,
 // scale factors two accumulators of 256 columns fill tensor memory, so a tile's epilogue runs under the next tile's
 // MMAs. Forward: CTA 0 stages 128 rows of G, CTA 1 the same 128 rows of U, so a CTA's accumulator holds g in columns
 // 0..127 and u in columns 128..255 of its own 128 tokens.
+// Maps: forward x, G, U (boxes of 128 rows); backward x, G, U, dg, du (boxes of 64 rows).
 template <int MODE, bool kBf16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Gated16Cfg::kThreads, 1)
-gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constant__ CUtensorMap tm_a1,
-    const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1, const Gated16Params p)
+gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_g,
+    const __grid_constant__ CUtensorMap tm_u, const __grid_constant__ CUtensorMap tm_dg, const __grid_constant__ CUtensorMap tm_du,
+    const Gated16Params p)
 {
     using C = Gated16Cfg;
     constexpr int S = C::kStages;
-    constexpr bool kAmn = MODE == G16_DW, kBmn = MODE != G16_GATED;
     extern __shared__ uint8_t smem_raw[];
     uint32_t const raw = smem_u32(smem_raw);
     uint32_t const base = (raw + 1023u) & ~1023u;
@@ -260,9 +268,9 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
         }
         *abort_flag = 0;
         mbar_fence_init();
-        prefetch_tensormap(&tm_a0);
-        prefetch_tensormap(&tm_b0);
-        prefetch_tensormap(&tm_b1);
+        prefetch_tensormap(&tm_x);
+        prefetch_tensormap(&tm_g);
+        prefetch_tensormap(&tm_u);
     }
     if (warp == 1) {
         tmem_alloc_pair(smem_u32(tmem_slot), C::kTmemCols);
@@ -276,32 +284,40 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
 
     int const pair = blockIdx.x >> 1;
     int const num_pairs = gridDim.x >> 1;
-    int const tiles = p.tiles_m * p.tiles_n;
-    int const items = tiles * p.splits;
+    int const items0 = p.first.tiles_m * p.first.tiles_n * p.first.splits;
+    int const items = items0 + (MODE == G16_BACKWARD ? p.second.tiles_m * p.second.tiles_n * p.second.splits : 0);
 
     struct Item {
         int tile_m, tile_n, split, kb0, kb1, half;
+        bool dw;
     };
     auto decode = [&](int t) {
         Item c;
+        bool const later = MODE == G16_BACKWARD && t >= items0;
+        Gated16Product const& q = later ? p.second : p.first;
+        c.dw = MODE == G16_BACKWARD && later == (p.first_is_dw == 0);
+        if (later) t -= items0;
+        int const tiles = q.tiles_m * q.tiles_n;
         c.split = t / tiles;
         int const r = t - c.split * tiles;
-        int const span = p.group_m * p.tiles_n;
+        int const span = q.group_m * q.tiles_n;
         int const g = r / span;
-        int const first = g * p.group_m;
-        int const gsz = min(p.group_m, p.tiles_m - first);
+        int const first = g * q.group_m;
+        int const gsz = min(q.group_m, q.tiles_m - first);
         int const in_g = r - g * span;
         c.tile_n = in_g / gsz;
         c.tile_m = first + (in_g - c.tile_n * gsz);
         c.half = 0;
-        if constexpr (MODE == G16_DW) {
-            c.half = c.tile_m >= p.tiles_half ? 1 : 0;
-            c.tile_m -= c.half * p.tiles_half;
+        if (c.dw) {
+            c.half = c.tile_m >= q.kb_half ? 1 : 0;
+            c.tile_m -= c.half * q.kb_half;
         }
-        c.kb0 = c.split * p.kb_per_split;
-        c.kb1 = min(p.kb_total, c.kb0 + p.kb_per_split);
+        c.kb0 = c.split * q.kb_per_split;
+        c.kb1 = min(q.kb_total, c.kb0 + q.kb_per_split);
         return c;
     };
+    griddep_launch_dependents();
+    griddep_wait();      // operands and outputs may be in use by the preceding kernel
 
     if (warp == 0) {
         // ------------------------------------------------------------------------------------ TMA producer (both CTAs)
@@ -312,7 +328,8 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
             for (int t = pair; ok && t < items; t += num_pairs) {
                 Item const c = decode(t);
                 int const a0 = c.tile_m * 256 + static_cast<int>(rank) * 128;
-                int const b0 = MODE == G16_GATED ? c.tile_n * 128 : c.tile_n * 256 + static_cast<int>(rank) * 128;
+                int const b0 = MODE == G16_FORWARD ? c.tile_n * 128 : c.tile_n * 256 + static_cast<int>(rank) * 128;
+                int const kb_half = MODE == G16_BACKWARD && !c.dw ? (p.first_is_dw ? p.second.kb_half : p.first.kb_half) : 0;
                 for (int kb = c.kb0; kb < c.kb1; ++kb) {
                     if (!wait_or_abort(empty_bar(stage), phase ^ 1u, abort_flag)) {
                         record_abort(FSO_DEV_WAIT_PRODUCER, abort_flag);
@@ -322,22 +339,24 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
                     uint32_t const fb = map_to_cta(full_bar(stage), 0);
                     if (leader) mbar_expect_tx(full_bar(stage), 2u * C::kStageBytes);
                     uint32_t const da = sA + stage * C::kOpBytes, db = sB + stage * C::kOpBytes;
-                    if constexpr (MODE == G16_GATED) {
-                        tma_load_2d_pair(da, &tm_a0, fb, kb * 64, a0);
-                        tma_load_2d_pair(db, rank == 0 ? &tm_b0 : &tm_b1, fb, kb * 64, b0);
-                    } else if constexpr (MODE == G16_DX) {
-                        bool const second = kb >= p.kb_half;
-                        int const kc = (second ? kb - p.kb_half : kb) * 64;
-                        const CUtensorMap* const tb = second ? &tm_b1 : &tm_b0;
-                        tma_load_2d_pair(da, second ? &tm_a1 : &tm_a0, fb, kc, a0);
+                    if constexpr (MODE == G16_FORWARD) {
+                        tma_load_2d_pair(da, &tm_x, fb, kb * 64, a0);
+                        tma_load_2d_pair(db, rank == 0 ? &tm_g : &tm_u, fb, kb * 64, b0);
+                    } else if (!c.dw) {
+                        bool const upper = kb >= kb_half;
+                        int const kc = (upper ? kb - kb_half : kb) * 64;
+                        const CUtensorMap* const ta = upper ? &tm_du : &tm_dg;
+                        const CUtensorMap* const tb = upper ? &tm_u : &tm_g;
+                        tma_load_2d_pair(da, ta, fb, kc, a0);
+                        tma_load_2d_pair(da + 8192, ta, fb, kc, a0 + 64);
                         tma_load_2d_pair(db, tb, fb, b0, kc);
                         tma_load_2d_pair(db + 8192, tb, fb, b0 + 64, kc);
                     } else {
-                        const CUtensorMap* const ta = c.half ? &tm_a1 : &tm_a0;
+                        const CUtensorMap* const ta = c.half ? &tm_du : &tm_dg;
                         tma_load_2d_pair(da, ta, fb, a0, kb * 64);
                         tma_load_2d_pair(da + 8192, ta, fb, a0 + 64, kb * 64);
-                        tma_load_2d_pair(db, &tm_b0, fb, b0, kb * 64);
-                        tma_load_2d_pair(db + 8192, &tm_b0, fb, b0 + 64, kb * 64);
+                        tma_load_2d_pair(db, &tm_x, fb, b0, kb * 64);
+                        tma_load_2d_pair(db + 8192, &tm_x, fb, b0 + 64, kb * 64);
                     }
                     if (++stage == S) {
                         stage = 0;
@@ -354,7 +373,6 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
             uint32_t phase = 0;
             int acc = 0;
             uint32_t acc_phase = 0;
-            constexpr uint32_t idesc = make_idesc_f16_pair(kBf16, kAmn, kBmn);
             bool ok = true;
             for (int t = pair; ok && t < items; t += num_pairs) {
                 Item const c = decode(t);
@@ -372,11 +390,14 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
                     }
                     tc_fence_after();
                     uint32_t const sa = sA + stage * C::kOpBytes, sb = sB + stage * C::kOpBytes;
-                    uint64_t const adesc = kAmn ? make_desc_mn_sw128(sa) : make_desc_sw128(sa);
+                    constexpr bool kBmn = MODE == G16_BACKWARD;
+                    uint64_t const adesc = c.dw ? make_desc_mn_sw128(sa) : make_desc_sw128(sa);
                     uint64_t const bdesc = kBmn ? make_desc_mn_sw128(sb) : make_desc_sw128(sb);
+                    uint32_t const idesc = make_idesc_f16_pair(kBf16, c.dw, kBmn);
+                    uint32_t const astep = c.dw ? 128u : 2u;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)      // 16 elements of the contraction: 32 bytes of a row, or 16 rows
-                        tc_mma_f16_pair(d_tmem, adesc + (kAmn ? 128u : 2u) * k, bdesc + (kBmn ? 128u : 2u) * k, idesc,
+                        tc_mma_f16_pair(d_tmem, adesc + astep * k, bdesc + (kBmn ? 128u : 2u) * k, idesc,
                             (kb > c.kb0 || k > 0) ? 1u : 0u);
                     tc_commit_pair_both(empty_bar(stage));
                     if (++stage == S) {
@@ -408,8 +429,9 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
             tc_fence_after();
             uint32_t const t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * 256);
             int const row = c.tile_m * 256 + static_cast<int>(rank) * 128 + quarter * 32 + lane;
-            bool const live = row < p.rows;
-            if constexpr (MODE == G16_GATED) {
+            Gated16Product const& q = MODE == G16_BACKWARD && c.dw == (p.first_is_dw == 0) ? p.second : p.first;
+            bool const live = row < q.rows;
+            if constexpr (MODE == G16_FORWARD) {
 #pragma unroll 1
                 for (int j = 0; j < 4; ++j) {
                     __syncwarp();      // lanes past the last row skip the stores below
@@ -419,15 +441,15 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
                     tmem_ld_32x16(t_row + 128 + in_tile, ru);
                     tmem_ld_wait();
                     int const col = c.tile_n * 128 + in_tile;
-                    if (!live || col >= p.cols) continue;
+                    if (!live || col >= q.cols) continue;
                     float g[16], u[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         g[i] = __uint_as_float(rg[i]);
                         u[i] = __uint_as_float(ru[i]);
                     }
-                    if (p.ws != nullptr) {
-                        float* const w = p.ws + (static_cast<int64_t>(c.split) * p.rows + row) * p.ws_cols + col;
+                    if (q.ws != nullptr) {
+                        float* const w = q.ws + (static_cast<int64_t>(c.split) * q.rows + row) * q.ws_cols + col;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             reinterpret_cast<float4*>(w)[i] = make_float4(g[4 * i], g[4 * i + 1], g[4 * i + 2], g[4 * i + 3]);
@@ -443,7 +465,7 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) g[i] = gate_value(g[i], p.act) * u[i];
-                    store_row16<kBf16>(p.out, static_cast<int64_t>(row) * p.ldo + col, g, p.cols - col, p.vec != 0);
+                    store_row16<kBf16>(q.out, static_cast<int64_t>(row) * q.ldo + col, g, q.cols - col, q.vec != 0);
                 }
             } else {
 #pragma unroll 1
@@ -454,20 +476,20 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_cons
                     tmem_ld_32x16(t_row + in_tile, r);
                     tmem_ld_wait();
                     int const col = c.tile_n * 256 + in_tile;
-                    if (!live || col >= p.cols) continue;
+                    if (!live || col >= q.cols) continue;
                     float v[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-                    if (p.ws != nullptr) {
-                        int64_t const slab = MODE == G16_DW ? 2 * c.split + c.half : c.split;
-                        float* const w = p.ws + (slab * p.rows + row) * p.ws_cols + col;
+                    if (q.ws != nullptr) {
+                        int64_t const slab = c.dw ? 2 * c.split + c.half : c.split;
+                        float* const w = q.ws + (slab * q.rows + row) * q.ws_cols + col;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             reinterpret_cast<float4*>(w)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                         continue;
                     }
-                    store_row16<kBf16>(p.out, c.half * p.out_half + static_cast<int64_t>(row) * p.ldo + col, v, p.cols - col,
-                        p.vec != 0);
+                    store_row16<kBf16>(q.out, c.half * q.out_half + static_cast<int64_t>(row) * q.ldo + col, v, q.cols - col,
+                        q.vec != 0);
                 }
             }
             tc_fence_before();
@@ -711,6 +733,8 @@ template <bool kBf16>
 __global__ void gated16_sum_kernel(float const* __restrict__ ws, int splits, int64_t slab, int64_t rows, int cols,
     int64_t ws_cols, uint16_t* __restrict__ out, int64_t ldo)
 {
+    griddep_launch_dependents();
+    griddep_wait();
     int const per_row = cols / 8;
     int64_t const i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= rows * per_row) return;
@@ -727,33 +751,48 @@ __global__ void gated16_sum_kernel(float const* __restrict__ ws, int splits, int
         pack16<kBf16>(v[4], v[5]), pack16<kBf16>(v[6], v[7]));
 }
 
-// The epilogue of the forward pass for a split contraction: sums, saved values, act and product. 16 columns a thread.
+// The epilogue of the forward pass for a split contraction: sums, saved values, act and product. Four columns a thread.
 template <bool kBf16>
 __global__ void gated16_finish_kernel(float const* __restrict__ ws, int splits, int rows, int cols, int64_t half_cols,
     int act, uint16_t* __restrict__ save_hi, uint8_t* __restrict__ save_lo, void* __restrict__ out, int vec)
 {
-    int const per_row = static_cast<int>(half_cols / 16);
+    griddep_launch_dependents();
+    griddep_wait();
+    int const per_row = static_cast<int>(half_cols / 4);
     int64_t const i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= static_cast<int64_t>(rows) * per_row) return;
     int64_t const row = i / per_row;
-    int const col = static_cast<int>(i - row * per_row) * 16;
-    float g[16] = {}, u[16] = {};
+    int const col = static_cast<int>(i - row * per_row) * 4;
+    float g[4] = {}, u[4] = {};
     for (int s = 0; s < splits; ++s) {
         float const* const w = ws + (static_cast<int64_t>(s) * rows + row) * 2 * half_cols + col;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            g[j] += w[j];
-            u[j] += w[half_cols + j];
-        }
+        float4 const a = *reinterpret_cast<float4 const*>(w), b = *reinterpret_cast<float4 const*>(w + half_cols);
+        g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
+        u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
     }
     if (save_hi != nullptr) {
         int64_t const at = row * 2 * half_cols + col;
-        store_saved(save_hi, save_lo, at, g);
-        store_saved(save_hi, save_lo, at + half_cols, u);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = to_24(h ? u[j] : g[j]);
+            *reinterpret_cast<uint2*>(save_hi + at + h * half_cols) =
+                make_uint2((b[0] >> 8) | ((b[1] >> 8) << 16), (b[2] >> 8) | ((b[3] >> 8) << 16));
+            *reinterpret_cast<uint32_t*>(save_lo + at + h * half_cols) =
+                (b[0] & 0xFFu) | ((b[1] & 0xFFu) << 8) | ((b[2] & 0xFFu) << 16) | (b[3] << 24);
+        }
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) g[j] = gate_value(g[j], act) * u[j];
-    store_row16<kBf16>(out, row * cols + col, g, cols - col, vec != 0);
+    for (int j = 0; j < 4; ++j) g[j] = gate_value(g[j], act) * u[j];
+    if (vec && col + 4 <= cols) {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + row * cols + col) =
+            make_uint2(pack16<kBf16>(g[0], g[1]), pack16<kBf16>(g[2], g[3]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col + j < cols) store16<kBf16>(out, row * cols + col + j, g[j]);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ dg and du
@@ -765,6 +804,8 @@ template <bool kBf16>
 __global__ void gated_slopes_kernel(const void* __restrict__ dh, int64_t ldh, int dh_vec, uint16_t const* __restrict__ save_hi,
     uint8_t const* __restrict__ save_lo, int rows, int cols, int64_t half_cols, int act, uint16_t* __restrict__ out)
 {
+    griddep_launch_dependents();
+    griddep_wait();
     int const per_row = static_cast<int>(half_cols / 8);
     int64_t const i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= static_cast<int64_t>(rows) * per_row) return;
@@ -836,66 +877,100 @@ inline int64_t gated_half_cols(int64_t inter) { return (inter + 15) / 16 * 16; }
 
 constexpr int kGatedRowsMax = 128;      // rows of x up to which the few-rows kernel runs the forward pass
 
-// Tiles and slices of one of the three products. Pure host arithmetic.
+// Tiles and slices of the products. Pure host arithmetic.
 struct Gated16Plan {
-    int tiles_m, tiles_half, tiles_n, kb, kb_half, splits, kb_per_split;
-    int64_t ws_bytes;
+    int tiles_m, tiles_n, kb, kb_half, splits, kb_per_split;
+    int64_t ws_bytes, ws_cols;
 };
 
-inline Gated16Plan plan_gated16(int mode, int64_t t, int64_t k, int64_t inter, int sms)
+inline int tiles_of(int64_t n, int64_t w) { return static_cast<int>((n + w - 1) / w); }
+
+inline Gated16Plan plan_gated16_forward(int64_t t, int64_t k, int64_t inter, int sms)
 {
     Gated16Plan p{};
-    auto tiles = [](int64_t n, int64_t w) { return static_cast<int>((n + w - 1) / w); };
-    int64_t rows = t, ws_cols = k;
-    if (mode == G16_GATED) {
-        if (t <= kGatedRowsMax) return p;      // no workspace
-        p.tiles_m = tiles(t, 256);
-        p.tiles_n = tiles(inter, 128);
-        p.kb = tiles(k, 64);
-        ws_cols = 2 * gated_half_cols(inter);
-    } else if (mode == G16_DX) {
-        p.tiles_m = tiles(t, 256);
-        p.tiles_n = tiles(k, 256);
-        p.kb_half = tiles(inter, 64);
-        p.kb = 2 * p.kb_half;
-        ws_cols = (k + 15) / 16 * 16;
-    } else {
-        p.tiles_half = tiles(inter, 256);
-        p.tiles_m = 2 * p.tiles_half;
-        p.tiles_n = tiles(k, 256);
-        p.kb = tiles(t, 64);
-        rows = 2 * inter;
-        ws_cols = (k + 15) / 16 * 16;
-    }
+    if (t <= kGatedRowsMax) return p;      // no workspace
+    p.tiles_m = tiles_of(t, 256);
+    p.tiles_n = tiles_of(inter, 128);
+    p.kb = tiles_of(k, 64);
+    p.ws_cols = 2 * gated_half_cols(inter);
     // slices of the contraction where the tiles would leave half of the SM pairs without work
     pick_splits(static_cast<int64_t>(p.tiles_m) * p.tiles_n, p.kb, sms / 2, 8, 16, &p.splits, &p.kb_per_split);
-    p.ws_bytes = p.splits > 1 ? p.splits * rows * ws_cols * 4 : 0;
+    p.ws_bytes = p.splits > 1 ? p.splits * t * p.ws_cols * 4 : 0;
     return p;
 }
 
+// The backward pass: dx and dW share the SM pairs. Where one of them has fewer tiles than there are pairs its contraction is
+// cut into slices of about a pair's part of all the work, of at least 512 elements, at most 16.
+inline void plan_gated16_backward(int64_t t, int64_t k, int64_t inter, bool need_x, bool need_w, int sms, Gated16Plan& dx,
+    Gated16Plan& dw)
+{
+    int const pairs = std::max(1, sms / 2);
+    dx = Gated16Plan{};
+    dw = Gated16Plan{};
+    dx.kb_half = tiles_of(inter, 64);
+    dx.kb = 2 * dx.kb_half;
+    dw.kb_half = tiles_of(inter, 256);
+    dw.kb = tiles_of(t, 64);
+    dx.tiles_n = dw.tiles_n = tiles_of(k, 256);
+    dx.tiles_m = need_x ? tiles_of(t, 256) : 0;
+    dw.tiles_m = need_w ? 2 * dw.kb_half : 0;
+    dx.ws_cols = dw.ws_cols = (k + 15) / 16 * 16;
+    int64_t const work = static_cast<int64_t>(dx.tiles_m) * dx.tiles_n * dx.kb + static_cast<int64_t>(dw.tiles_m) * dw.tiles_n * dw.kb;
+    int const share = static_cast<int>(std::max<int64_t>(8, std::min<int64_t>(work / pairs, 1 << 24)));
+    for (Gated16Plan* p : {&dx, &dw}) {
+        p->splits = 1;
+        if (static_cast<int64_t>(p->tiles_m) * p->tiles_n < pairs && p->kb > share)
+            p->splits = std::min(16, tiles_of(p->kb, share));
+        p->kb_per_split = tiles_of(p->kb, p->splits);
+        p->splits = tiles_of(p->kb, p->kb_per_split);
+        int64_t const rows = p == &dx ? t : 2 * inter;
+        p->ws_bytes = p->splits > 1 && p->tiles_m > 0 ? p->splits * rows * p->ws_cols * 4 : 0;
+    }
+}
+
+// Launch with programmatic dependent launch: every kernel of this file lets its successor start early and waits for its own
+// predecessor before it touches memory.
+template <typename... Params, typename... Args>
+inline int launch_chained(const char* what, void (*kernel)(Params...), unsigned grid, int threads, int smem, cudaStream_t stream,
+    Args const&... args)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_attribute(&attr[0]);
+    FSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
+    return launch_status(what);
+}
+
 template <int MODE, bool kBf16>
-inline int launch_gated16(CUtensorMap const (&m)[4], Gated16Params const& p, int sms, cudaStream_t stream)
+inline int launch_gated16(CUtensorMap const (&m)[5], Gated16Params const& p, int sms, cudaStream_t stream)
 {
     static std::atomic<uint64_t> done{0};
     auto kernel = gated16_pair_kernel<MODE, kBf16>;
     int const rc = ensure_smem_attr(kernel, Gated16Cfg::kSmemBytes, done);
     if (rc != 0) return rc;
-    int64_t const items = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
-    int const pairs = static_cast<int>(std::min<int64_t>(items, std::max(1, sms / 2)));
-    kernel<<<2 * pairs, Gated16Cfg::kThreads, Gated16Cfg::kSmemBytes, stream>>>(m[0], m[1], m[2], m[3], p);
-    return launch_status("gated16_pair_kernel");
+    int64_t const items = static_cast<int64_t>(p.first.tiles_m) * p.first.tiles_n * p.first.splits
+        + static_cast<int64_t>(p.second.tiles_m) * p.second.tiles_n * p.second.splits;
+    FSO_REQUIRE(items < (1ll << 31), "gated projection: %lld tiles are beyond the kernel's index range", static_cast<long long>(items));
+    unsigned const pairs = static_cast<unsigned>(std::min<int64_t>(items, std::max(1, sms / 2)));
+    return launch_chained("gated16_pair_kernel", kernel, 2 * pairs, Gated16Cfg::kThreads, Gated16Cfg::kSmemBytes, stream, m[0], m[1],
+        m[2], m[3], m[4], p);
 }
 
-inline void fill_gated16(Gated16Params& p, Gated16Plan const& pl)
+inline void fill_product(Gated16Product& q, Gated16Plan const& pl)
 {
-    p.tiles_m = pl.tiles_m;
-    p.tiles_half = pl.tiles_half;
-    p.tiles_n = pl.tiles_n;
-    p.group_m = std::min(pl.tiles_m, 8);
-    p.kb_total = pl.kb;
-    p.kb_half = pl.kb_half;
-    p.splits = pl.splits;
-    p.kb_per_split = pl.kb_per_split;
+    q.tiles_m = pl.tiles_m;
+    q.tiles_n = pl.tiles_n;
+    q.group_m = std::max(1, std::min(pl.tiles_m, 8));
+    q.kb_total = pl.kb;
+    q.kb_half = pl.kb_half;
+    q.splits = pl.splits;
+    q.kb_per_split = pl.kb_per_split;
+    q.ws_cols = pl.ws_cols;
 }
 
 inline unsigned blocks_for(int64_t threads, int per_block) { return static_cast<unsigned>((threads + per_block - 1) / per_block); }
@@ -962,110 +1037,100 @@ inline int gated_forward(const void* x, int64_t ldx, const void* gate_up, void* 
                        : launch_gated_rows<128, kBf16>(x, ldx, gate_up, k, r, stream);
     }
     int const sms = sm_count();
-    Gated16Plan const pl = plan_gated16(G16_GATED, t, k, inter, sms);
-    CUtensorMap m[4];
+    Gated16Plan const pl = plan_gated16_forward(t, k, inter, sms);
+    CUtensorMap m[5];
     uint16_t const* const w = static_cast<uint16_t const*>(gate_up);
     int rc = make_map16(&m[0], x, t, k, ldx, 128);
-    if (rc == 0) rc = make_map16(&m[2], w, inter, k, k, 128);
-    if (rc == 0) rc = make_map16(&m[3], w + inter * k, inter, k, k, 128);
+    if (rc == 0) rc = make_map16(&m[1], w, inter, k, k, 128);
+    if (rc == 0) rc = make_map16(&m[2], w + inter * k, inter, k, k, 128);
     if (rc != 0) return rc;
-    m[1] = m[0];
+    m[3] = m[4] = m[0];
     Gated16Params p{};
-    fill_gated16(p, pl);
-    p.rows = static_cast<int>(t);
-    p.cols = static_cast<int>(inter);
+    fill_product(p.first, pl);
+    p.first.rows = static_cast<int>(t);
+    p.first.cols = static_cast<int>(inter);
+    p.first.vec = inter % 8 == 0 && aligned16(h);
+    p.first.out = h;
+    p.first.ldo = inter;
+    p.first.ws = pl.splits > 1 ? static_cast<float*>(ws) : nullptr;
     p.act = act;
-    p.vec = inter % 8 == 0 && aligned16(h);
-    p.out = h;
-    p.ldo = inter;
     p.save_hi = static_cast<uint16_t*>(save_hi);
     p.save_lo = static_cast<uint8_t*>(save_lo);
     p.half_cols = gated_half_cols(inter);
-    p.ws = pl.splits > 1 ? static_cast<float*>(ws) : nullptr;
-    p.ws_cols = 2 * p.half_cols;
-    rc = launch_gated16<G16_GATED, kBf16>(m, p, sms, stream);
+    rc = launch_gated16<G16_FORWARD, kBf16>(m, p, sms, stream);
     if (rc != 0 || pl.splits == 1) return rc;
-    gated16_finish_kernel<kBf16><<<blocks_for(t * (p.half_cols / 16), 128), 128, 0, stream>>>(p.ws, pl.splits, p.rows, p.cols,
-        p.half_cols, act, p.save_hi, p.save_lo, h, p.vec);
-    return launch_status("gated16_finish_kernel");
+    return launch_chained("gated16_finish_kernel", gated16_finish_kernel<kBf16>, blocks_for(t * (p.half_cols / 4), 128), 128, 0,
+        stream, p.first.ws, pl.splits, p.first.rows, p.first.cols, p.half_cols, act, p.save_hi, p.save_lo, h, p.first.vec);
 }
 
-// Workspace of the backward pass: dg and du (16 bit [T, 2 * half_cols]), then the slices of whichever product has them.
+// Workspace of the backward pass: dg and du (16 bit [T, 2 * half_cols]), then the slices of dx and of dW. Enough for one
+// gradient alone as well as for both.
+inline int64_t gated_slopes_bytes(int64_t t, int64_t inter) { return (t * 2 * gated_half_cols(inter) * 2 + 255) / 256 * 256; }
+
 inline int64_t gated_backward_ws_bytes(int64_t t, int64_t k, int64_t inter, int sms)
 {
-    int64_t const slopes = (t * 2 * gated_half_cols(inter) * 2 + 255) / 256 * 256;
-    return slopes + std::max(plan_gated16(G16_DX, t, k, inter, sms).ws_bytes, plan_gated16(G16_DW, t, k, inter, sms).ws_bytes);
+    int64_t sums = 0;
+    for (int need = 1; need < 4; ++need) {
+        Gated16Plan dx, dw;
+        plan_gated16_backward(t, k, inter, need & 1, need & 2, sms, dx, dw);
+        sums = std::max(sums, (dx.ws_bytes + 255) / 256 * 256 + dw.ws_bytes);
+    }
+    return gated_slopes_bytes(t, inter) + sums;
 }
 
 template <bool kBf16>
 inline int gated_backward(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* gate_up, const void* save_hi,
     const void* save_lo, void* dx, void* dgate_up, int64_t t, int64_t k, int64_t inter, int act, void* ws, cudaStream_t stream)
 {
+    if (dx == nullptr && dgate_up == nullptr) return 0;
     int const sms = sm_count();
     int64_t const hc = gated_half_cols(inter);
     uint16_t* const slopes = static_cast<uint16_t*>(ws);
-    float* const sums = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + (t * 2 * hc * 2 + 255) / 256 * 256);
     int const dh_vec = inter % 8 == 0 && ldh % 8 == 0 && aligned16(dh);
-    gated_slopes_kernel<kBf16><<<blocks_for(t * (hc / 8), 256), 256, 0, stream>>>(dh, ldh, dh_vec,
-        static_cast<uint16_t const*>(save_hi), static_cast<uint8_t const*>(save_lo), static_cast<int>(t),
+    int rc = launch_chained("gated_slopes_kernel", gated_slopes_kernel<kBf16>, blocks_for(t * (hc / 8), 256), 256, 0, stream, dh, ldh,
+        dh_vec, static_cast<uint16_t const*>(save_hi), static_cast<uint8_t const*>(save_lo), static_cast<int>(t),
         static_cast<int>(inter), hc, act, slopes);
-    int rc = launch_status("gated_slopes_kernel");
     if (rc != 0) return rc;
+
+    Gated16Plan px, pw;
+    plan_gated16_backward(t, k, inter, dx != nullptr, dgate_up != nullptr, sms, px, pw);
+    float* const sums_x = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + gated_slopes_bytes(t, inter));
+    float* const sums_w = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sums_x) + (px.ws_bytes + 255) / 256 * 256);
     uint16_t const* const w = static_cast<uint16_t const*>(gate_up);
-    if (dx != nullptr) {
-        Gated16Plan const pl = plan_gated16(G16_DX, t, k, inter, sms);
-        CUtensorMap m[4];
-        rc = make_map16(&m[0], slopes, t, inter, 2 * hc, 128);
-        if (rc == 0) rc = make_map16(&m[1], slopes + hc, t, inter, 2 * hc, 128);
-        if (rc == 0) rc = make_map16(&m[2], w, inter, k, k, 64);
-        if (rc == 0) rc = make_map16(&m[3], w + inter * k, inter, k, k, 64);
-        if (rc != 0) return rc;
-        Gated16Params p{};
-        fill_gated16(p, pl);
-        p.rows = static_cast<int>(t);
-        p.cols = static_cast<int>(k);
-        p.vec = 1;
-        p.out = dx;
-        p.ldo = k;
-        p.ws = pl.splits > 1 ? sums : nullptr;
-        p.ws_cols = (k + 15) / 16 * 16;
-        rc = launch_gated16<G16_DX, kBf16>(m, p, sms, stream);
-        if (rc != 0) return rc;
-        if (pl.splits > 1) {
-            gated16_sum_kernel<kBf16><<<blocks_for(t * (k / 8), 256), 256, 0, stream>>>(sums, pl.splits, t * p.ws_cols, t,
-                p.cols, p.ws_cols, static_cast<uint16_t*>(dx), k);
-            rc = launch_status("gated16_sum_kernel");
-            if (rc != 0) return rc;
-        }
-    }
-    if (dgate_up != nullptr) {
-        Gated16Plan const pl = plan_gated16(G16_DW, t, k, inter, sms);
-        CUtensorMap m[4];
-        rc = make_map16(&m[0], slopes, t, inter, 2 * hc, 64);
-        if (rc == 0) rc = make_map16(&m[1], slopes + hc, t, inter, 2 * hc, 64);
-        if (rc == 0) rc = make_map16(&m[2], x, t, k, ldx, 64);
-        if (rc != 0) return rc;
-        m[3] = m[2];
-        Gated16Params p{};
-        fill_gated16(p, pl);
-        p.rows = static_cast<int>(inter);
-        p.cols = static_cast<int>(k);
-        p.vec = 1;
-        p.out = dgate_up;
-        p.ldo = k;
-        p.out_half = inter * k;
-        p.ws = pl.splits > 1 ? sums : nullptr;
-        p.ws_cols = (k + 15) / 16 * 16;
-        rc = launch_gated16<G16_DW, kBf16>(m, p, sms, stream);
-        if (rc != 0) return rc;
-        if (pl.splits > 1) {
-            gated16_sum_kernel<kBf16><<<blocks_for(2 * inter * (k / 8), 256), 256, 0, stream>>>(sums, pl.splits,
-                2 * inter * p.ws_cols, 2 * inter, p.cols, p.ws_cols, static_cast<uint16_t*>(dgate_up), k);
-            rc = launch_status("gated16_sum_kernel");
-            if (rc != 0) return rc;
-        }
-    }
-    return 0;
+    CUtensorMap m[5];
+    rc = make_map16(&m[0], x, t, k, ldx, 64);
+    if (rc == 0) rc = make_map16(&m[1], w, inter, k, k, 64);
+    if (rc == 0) rc = make_map16(&m[2], w + inter * k, inter, k, k, 64);
+    if (rc == 0) rc = make_map16(&m[3], slopes, t, inter, 2 * hc, 64);
+    if (rc == 0) rc = make_map16(&m[4], slopes + hc, t, inter, 2 * hc, 64);
+    if (rc != 0) return rc;
+    Gated16Params p{};
+    p.first_is_dw = pw.kb_per_split > px.kb_per_split;      // long tiles first: the short ones even out the last round
+    Gated16Product& qx = p.first_is_dw ? p.second : p.first;
+    Gated16Product& qw = p.first_is_dw ? p.first : p.second;
+    fill_product(qx, px);
+    qx.rows = static_cast<int>(t);
+    qx.cols = static_cast<int>(k);
+    qx.vec = 1;
+    qx.out = dx;
+    qx.ldo = k;
+    qx.ws = px.splits > 1 ? sums_x : nullptr;
+    fill_product(qw, pw);
+    qw.rows = static_cast<int>(inter);
+    qw.cols = static_cast<int>(k);
+    qw.vec = 1;
+    qw.out = dgate_up;
+    qw.ldo = k;
+    qw.out_half = inter * k;
+    qw.ws = pw.splits > 1 ? sums_w : nullptr;
+    rc = launch_gated16<G16_BACKWARD, kBf16>(m, p, sms, stream);
+    if (rc == 0 && dx != nullptr && px.splits > 1)
+        rc = launch_chained("gated16_sum_kernel", gated16_sum_kernel<kBf16>, blocks_for(t * (k / 8), 256), 256, 0, stream, sums_x,
+            px.splits, t * px.ws_cols, t, static_cast<int>(k), px.ws_cols, static_cast<uint16_t*>(dx), k);
+    if (rc == 0 && dgate_up != nullptr && pw.splits > 1)
+        rc = launch_chained("gated16_sum_kernel", gated16_sum_kernel<kBf16>, blocks_for(2 * inter * (k / 8), 256), 256, 0, stream,
+            sums_w, pw.splits, 2 * inter * pw.ws_cols, 2 * inter, static_cast<int>(k), pw.ws_cols, static_cast<uint16_t*>(dgate_up), k);
+    return rc;
 }
 
 }  // namespace fso

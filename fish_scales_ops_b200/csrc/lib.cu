@@ -698,7 +698,7 @@ int fso_gated_linear_ws_bytes(int64_t t, int64_t k, int64_t inter, int64_t* byte
     FSO_REQUIRE(bytes != nullptr, "fso_gated_linear_ws_bytes: bytes is NULL");
     int const rc = check_gated_shape("fso_gated_linear_ws_bytes", t, k, inter, 0, 0);
     if (rc != 0) return rc;
-    *bytes = t == 0 ? 0 : plan_gated16(G16_GATED, t, k, inter, sm_count()).ws_bytes;
+    *bytes = t == 0 ? 0 : plan_gated16_forward(t, k, inter, sm_count()).ws_bytes;
     return 0;
 }
 
@@ -714,7 +714,7 @@ int fso_gated_linear(const void* x, int64_t ldx, const void* gate_up, void* h, v
         static_cast<long long>(ldx));
     FSO_REQUIRE(aligned16(x) && aligned16(gate_up) && aligned16(save_hi) && aligned16(save_lo) && aligned16(ws),
         "fso_gated_linear: x, gate_up, the saved arrays and the workspace must be 16-byte aligned");
-    int64_t const need = plan_gated16(G16_GATED, t, k, inter, sm_count()).ws_bytes;
+    int64_t const need = plan_gated16_forward(t, k, inter, sm_count()).ws_bytes;
     FSO_REQUIRE(need == 0 || (ws != nullptr && ws_bytes >= need), "fso_gated_linear: workspace of %lld bytes required, got %lld",
         static_cast<long long>(need), static_cast<long long>(ws == nullptr ? 0 : ws_bytes));
     return dtype == 0 ? gated_forward<true>(x, ldx, gate_up, h, save_hi, save_lo, t, k, inter, static_cast<int>(activation), ws, as_stream(stream))

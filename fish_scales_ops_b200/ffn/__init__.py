@@ -138,9 +138,15 @@ class _GatedLinear(torch.autograd.Function):
         return h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
+        if torch.is_grad_enabled():      # create_graph: the gradients come with a node that refuses to be differentiated
+            return _differentiable_once(ctx, dh)
         return (*_gradients(_eager_backward, ctx, dh), None)
+
+
+@torch.autograd.function.once_differentiable
+def _differentiable_once(ctx, dh):
+    return (*_gradients(_eager_backward, ctx, dh), None)
 
 
 def _eager_backward(dh, x, gate_up, hi, lo, activation, need_x, need_w):
