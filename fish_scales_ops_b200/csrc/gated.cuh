@@ -14,6 +14,7 @@
 // bytes below that.
 #pragma once
 
+#include <cmath>
 #include <cuda_fp16.h>
 
 #include "gemm_host.cuh"
@@ -29,7 +30,8 @@ struct Gated16Cfg {
     static constexpr int kThreads = 128 + 32 * kEpiWarps;
     static constexpr int kOpBytes = 128 * 128;          // one operand of one CTA and stage: 128 rows x 64 elements
     static constexpr int kStageBytes = 2 * kOpBytes;
-    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 512;
+    static constexpr int kTurnBytes = 32 * 128;         // of each epilogue warp: 32 rows x 128 bytes on their way out
+    static constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kTurnBytes + 1024 + 512;
     static constexpr int kTmemCols = 512;               // two accumulators of 256 columns
     static_assert(kSmemBytes <= 227 * 1024 && kSmemBytes > 116 * 1024, "one CTA per SM");
 };
@@ -146,42 +148,62 @@ __device__ __forceinline__ uint32_t to_24(float v)
 
 __device__ __forceinline__ float from_24(uint32_t hi, uint32_t lo) { return __uint_as_float((hi << 16) | (lo << 8)); }
 
-// 16 consecutive fp32 values of one row, the first `valid` of them inside the row, to 16 bits.
-template <bool kBf16>
-__device__ __forceinline__ void store_row16(void* out, int64_t at, float const (&v)[16], int valid, bool vec)
+// A tile of 32 rows x 16 * kChunks bytes turns in a warp's shared memory: it is held a row to a lane and leaves with
+// neighbouring lanes on neighbouring 16-byte chunks of a row, so that whole sectors are written. Chunks are xor-ed with the row:
+// both sides of the turn hit all banks.
+template <int kChunks>
+__device__ __forceinline__ void turn_put(uint32_t turn, int lane, int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
-    if (vec) {      // rows start on 16-byte boundaries and `at` is a multiple of 16 inside the row
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            if (8 * q + 8 <= valid) {
-                uint4 const w = make_uint4(pack16<kBf16>(v[8 * q], v[8 * q + 1]), pack16<kBf16>(v[8 * q + 2], v[8 * q + 3]),
-                    pack16<kBf16>(v[8 * q + 4], v[8 * q + 5]), pack16<kBf16>(v[8 * q + 6], v[8 * q + 7]));
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at + 8 * q) = w;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (j < valid) store16<kBf16>(out, at + j, v[j]);
-    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(turn + lane * (16 * kChunks) + ((chunk ^ ((lane * kChunks / 8) & (kChunks - 1))) << 4)), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
 }
 
-// 16 consecutive g (or u) values of one row to the saved arrays, whose rows are padded to multiples of 16 columns.
-__device__ __forceinline__ void store_saved(uint16_t* hi, uint8_t* lo, int64_t at, float const (&v)[16])
+// Calls to(row, chunk, value) for every chunk of the first `rows` rows.
+template <int kChunks, typename To>
+__device__ __forceinline__ void turn_out(uint32_t turn, int lane, int rows, To to)
 {
-    uint32_t h[8], l[4];
+    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        uint32_t const a = to_24(v[2 * j]), b = to_24(v[2 * j + 1]);
-        h[j] = (a >> 8) | ((b >> 8) << 16);
-        uint32_t const two = (a & 0xFFu) | ((b & 0xFFu) << 8);
-        if (j & 1) l[j >> 1] |= two << 16;
-        else l[j >> 1] = two;
+    for (int i = 0; i < kChunks; ++i) {
+        int const row = i * (32 / kChunks) + lane / kChunks, chunk = lane % kChunks;
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(turn + row * (16 * kChunks) + ((chunk ^ ((row * kChunks / 8) & (kChunks - 1))) << 4))
+                     : "memory");
+        if (row < rows) to(row, chunk, v);
     }
-    uint4* const dh = reinterpret_cast<uint4*>(hi + at);
-    dh[0] = make_uint4(h[0], h[1], h[2], h[3]);
-    dh[1] = make_uint4(h[4], h[5], h[6], h[7]);
-    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    __syncwarp();
+}
+
+// Four neighbouring g and u of one row: saved values (rows padded to multiples of 16 columns), act and product. `valid`: how
+// many of them lie inside the row of the output.
+template <bool kBf16>
+__device__ __forceinline__ void finish_four(float (&g)[4], float (&u)[4], int act, uint16_t* hi, uint8_t* lo, int64_t at,
+    int64_t half_cols, void* out, int64_t to, int valid, bool vec)
+{
+    if (hi != nullptr) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = to_24(h ? u[j] : g[j]);
+            *reinterpret_cast<uint2*>(hi + at + h * half_cols) =
+                make_uint2((b[0] >> 8) | ((b[1] >> 8) << 16), (b[2] >> 8) | ((b[3] >> 8) << 16));
+            *reinterpret_cast<uint32_t*>(lo + at + h * half_cols) =
+                (b[0] & 0xFFu) | ((b[1] & 0xFFu) << 8) | ((b[2] & 0xFFu) << 16) | (b[3] << 24);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = gate_value(g[j], act) * u[j];
+    if (vec && valid >= 4) {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + to) = make_uint2(pack16<kBf16>(g[0], g[1]), pack16<kBf16>(g[2], g[3]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < valid) store16<kBf16>(out, to + j, g[j]);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ tensor-core forms
@@ -243,12 +265,13 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     uint8_t* const gbase = smem_raw + (base - raw);
     uint32_t const sA = base;
     uint32_t const sB = sA + S * C::kOpBytes;
-    uint32_t const bars = sB + S * C::kOpBytes;
+    uint32_t const sTurn = sB + S * C::kOpBytes;
+    uint32_t const bars = sTurn + C::kEpiWarps * C::kTurnBytes;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
     auto tfull_bar = [&](int a) { return bars + 8u * (2 * S + a); };
     auto tempty_bar = [&](int a) { return bars + 8u * (2 * S + 2 + a); };
-    uint32_t const misc_off = static_cast<uint32_t>(S) * C::kStageBytes + 8u * (2 * S + 4);
+    uint32_t const misc_off = static_cast<uint32_t>(S) * C::kStageBytes + C::kEpiWarps * C::kTurnBytes + 8u * (2 * S + 4);
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + misc_off);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(gbase + misc_off + 4);
 
@@ -426,70 +449,119 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                 if (lane == 0) record_abort(FSO_DEV_WAIT_EPILOGUE, abort_flag);
                 break;
             }
+            __syncwarp();      // the loads from tensor memory below are the whole warp's
             tc_fence_after();
             uint32_t const t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * 256);
-            int const row = c.tile_m * 256 + static_cast<int>(rank) * 128 + quarter * 32 + lane;
             Gated16Product const& q = MODE == G16_BACKWARD && c.dw == (p.first_is_dw == 0) ? p.second : p.first;
-            bool const live = row < q.rows;
+            int const row0 = c.tile_m * 256 + static_cast<int>(rank) * 128 + quarter * 32;      // of this warp
+            int const rows = min(32, q.rows - row0);
+            uint32_t const turn = sTurn + (warp - 4) * C::kTurnBytes;
             if constexpr (MODE == G16_FORWARD) {
 #pragma unroll 1
-                for (int j = 0; j < 4; ++j) {
-                    __syncwarp();      // lanes past the last row skip the stores below
-                    int const in_tile = half * 64 + 16 * j;
-                    uint32_t rg[16], ru[16];
-                    tmem_ld_32x16(t_row + in_tile, rg);
-                    tmem_ld_32x16(t_row + 128 + in_tile, ru);
-                    tmem_ld_wait();
+                for (int j = 0; j < 2; ++j) {
+                    int const in_tile = half * 64 + 32 * j;
                     int const col = c.tile_n * 128 + in_tile;
-                    if (!live || col >= q.cols) continue;
-                    float g[16], u[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        g[i] = __uint_as_float(rg[i]);
-                        u[i] = __uint_as_float(ru[i]);
-                    }
+                    if (col >= q.cols || rows <= 0) break;
+                    float g[32], u[32];
+                    tmem_ld_32x32(t_row + in_tile, reinterpret_cast<uint32_t(&)[32]>(g));
+                    tmem_ld_32x32(t_row + 128 + in_tile, reinterpret_cast<uint32_t(&)[32]>(u));
+                    tmem_ld_wait();
+                    // columns that exist from `col` on: of the arrays padded to 16, and of the output
+                    int const padded = min(32, static_cast<int>(p.half_cols) - col), valid = min(32, q.cols - col);
                     if (q.ws != nullptr) {
-                        float* const w = q.ws + (static_cast<int64_t>(c.split) * q.rows + row) * q.ws_cols + col;
+                        float* const w = q.ws + (static_cast<int64_t>(c.split) * q.rows + row0) * q.ws_cols + col;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            reinterpret_cast<float4*>(w)[i] = make_float4(g[4 * i], g[4 * i + 1], g[4 * i + 2], g[4 * i + 3]);
-                            reinterpret_cast<float4*>(w + p.half_cols)[i] =
-                                make_float4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+                        for (int h = 0; h < 2; ++h) {
+                            float const (&v)[32] = h ? u : g;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                turn_put<8>(turn, lane, i, __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                                    __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+                            turn_out<8>(turn, lane, rows, [&](int r, int i, uint4 x) {
+                                if (4 * i < padded) *reinterpret_cast<uint4*>(w + r * q.ws_cols + h * p.half_cols + 4 * i) = x;
+                            });
                         }
                         continue;
                     }
                     if (p.save_hi != nullptr) {
-                        int64_t const at = static_cast<int64_t>(row) * 2 * p.half_cols + col;
-                        store_saved(p.save_hi, p.save_lo, at, g);
-                        store_saved(p.save_hi, p.save_lo, at + p.half_cols, u);
+                        int64_t const at = static_cast<int64_t>(row0) * 2 * p.half_cols + col;
+                        uint32_t low[16];      // lower bytes of g, then of u
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float const (&v)[32] = h ? u : g;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                uint32_t b[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) b[e] = to_24(v[8 * i + e]);
+                                turn_put<8>(turn, lane, 4 * h + i, (b[0] >> 8) | ((b[1] >> 8) << 16), (b[2] >> 8) | ((b[3] >> 8) << 16),
+                                    (b[4] >> 8) | ((b[5] >> 8) << 16), (b[6] >> 8) | ((b[7] >> 8) << 16));
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                    low[8 * h + 2 * i + e] = (b[4 * e] & 0xFFu) | ((b[4 * e + 1] & 0xFFu) << 8)
+                                        | ((b[4 * e + 2] & 0xFFu) << 16) | (b[4 * e + 3] << 24);
+                            }
+                        }
+                        turn_out<8>(turn, lane, rows, [&](int r, int i, uint4 x) {
+                            if (8 * (i & 3) < padded)
+                                *reinterpret_cast<uint4*>(p.save_hi + at + r * 2 * p.half_cols + (i >> 2) * p.half_cols + 8 * (i & 3)) = x;
+                        });
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            turn_put<4>(turn, lane, i, low[4 * i], low[4 * i + 1], low[4 * i + 2], low[4 * i + 3]);
+                        turn_out<4>(turn, lane, rows, [&](int r, int i, uint4 x) {
+                            if (16 * (i & 1) < padded)
+                                *reinterpret_cast<uint4*>(p.save_lo + at + r * 2 * p.half_cols + (i >> 1) * p.half_cols + 16 * (i & 1)) = x;
+                        });
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) g[i] = gate_value(g[i], p.act) * u[i];
-                    store_row16<kBf16>(q.out, static_cast<int64_t>(row) * q.ldo + col, g, q.cols - col, q.vec != 0);
+                    for (int i = 0; i < 32; ++i) g[i] = gate_value(g[i], p.act) * u[i];
+                    if (q.vec) {
+                        uint16_t* const to = static_cast<uint16_t*>(q.out) + static_cast<int64_t>(row0) * q.ldo + col;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            turn_put<4>(turn, lane, i, pack16<kBf16>(g[8 * i], g[8 * i + 1]), pack16<kBf16>(g[8 * i + 2], g[8 * i + 3]),
+                                pack16<kBf16>(g[8 * i + 4], g[8 * i + 5]), pack16<kBf16>(g[8 * i + 6], g[8 * i + 7]));
+                        turn_out<4>(turn, lane, rows, [&](int r, int i, uint4 x) {
+                            if (8 * i < valid) *reinterpret_cast<uint4*>(to + r * q.ldo + 8 * i) = x;
+                        });
+                    } else if (lane < rows) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i < valid) store16<kBf16>(q.out, static_cast<int64_t>(row0 + lane) * q.ldo + col + i, g[i]);
+                    }
+                    __syncwarp();
                 }
             } else {
 #pragma unroll 1
-                for (int j = 0; j < 8; ++j) {
-                    __syncwarp();
-                    int const in_tile = half * 128 + 16 * j;
-                    uint32_t r[16];
-                    tmem_ld_32x16(t_row + in_tile, r);
-                    tmem_ld_wait();
+                for (int j = 0; j < 4; ++j) {
+                    int const in_tile = half * 128 + 32 * j;
                     int const col = c.tile_n * 256 + in_tile;
-                    if (!live || col >= q.cols) continue;
-                    float v[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+                    if (col >= q.cols || rows <= 0) break;
+                    float v[32];
+                    tmem_ld_32x32(t_row + in_tile, reinterpret_cast<uint32_t(&)[32]>(v));
+                    tmem_ld_wait();
+                    int const valid = min(32, q.cols - col);      // a multiple of 8: so is K
                     if (q.ws != nullptr) {
                         int64_t const slab = c.dw ? 2 * c.split + c.half : c.split;
-                        float* const w = q.ws + (slab * q.rows + row) * q.ws_cols + col;
+                        float* const w = q.ws + (slab * q.rows + row0) * q.ws_cols + col;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            reinterpret_cast<float4*>(w)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        for (int i = 0; i < 8; ++i)
+                            turn_put<8>(turn, lane, i, __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                                __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+                        turn_out<8>(turn, lane, rows, [&](int r, int i, uint4 x) {
+                            if (4 * i < valid) *reinterpret_cast<uint4*>(w + r * q.ws_cols + 4 * i) = x;
+                        });
                         continue;
                     }
-                    store_row16<kBf16>(q.out, c.half * q.out_half + static_cast<int64_t>(row) * q.ldo + col, v, q.cols - col,
-                        q.vec != 0);
+                    uint16_t* const to = static_cast<uint16_t*>(q.out) + c.half * q.out_half + static_cast<int64_t>(row0) * q.ldo + col;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        turn_put<4>(turn, lane, i, pack16<kBf16>(v[8 * i], v[8 * i + 1]), pack16<kBf16>(v[8 * i + 2], v[8 * i + 3]),
+                            pack16<kBf16>(v[8 * i + 4], v[8 * i + 5]), pack16<kBf16>(v[8 * i + 6], v[8 * i + 7]));
+                    turn_out<4>(turn, lane, rows, [&](int r, int i, uint4 x) {
+                        if (8 * i < valid) *reinterpret_cast<uint4*>(to + r * q.ldo + 8 * i) = x;
+                    });
                 }
             }
             tc_fence_before();
@@ -519,10 +591,11 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
 
 // ------------------------------------------------------------------------------------------------ few rows
 //
-// The forward pass for at most 128 rows of x, where the weight bytes are the cost: 64 rows of G and the same 64 rows of U on
-// MMA-M, the rows of x on MMA-N, one tile for each CTA and two CTAs to an SM, so that more than a hundred kilobytes of
-// an SM's weights are on their way at any time. Where the tiles leave SMs without work the CTAs of a cluster split the
-// contraction, and each adds up its part of the outputs over distributed shared memory, in a fixed order.
+// The forward pass where 256 x 256 tiles are too coarse: 64 rows of G and the same 64 rows of U on MMA-M, up to 256 rows of x
+// (a multiple of 16) on MMA-N, one tile for each CTA. Up to 128 rows the weight bytes are the cost, and two CTAs share
+// an SM, so that more than a hundred kilobytes of its weights are on their way at any time. Where the tiles leave SMs
+// without work the CTAs of a cluster split the contraction, and each adds up its part of the outputs over distributed
+// shared memory, in a fixed order.
 // Nothing is read before the preceding kernel has finished: unlike a prepared weight, gate_up may be its output.
 template <int BN>
 struct GatedRowsCfg {
@@ -530,17 +603,20 @@ struct GatedRowsCfg {
     static constexpr int kABytes = 128 * 128;
     static constexpr int kBBytes = BN * 128;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = (110 * 1024) / kStageBytes;
+    static constexpr int kBlocks = BN <= 128 ? 2 : 1;      // CTAs that share an SM
+    static constexpr int kStages = (220 * 1024 / kBlocks) / kStageBytes;
     static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
     static constexpr int kRedStride = 132;     // floats between the rows of x in the sums of a slice
     static constexpr int kTmemCols = BN < 32 ? 32 : BN;
-    static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
+    static_assert(kBlocks * (kSmemBytes + 1024) <= 228 * 1024, "CTAs of an SM");
     static_assert(BN * kRedStride * 4 <= kStages * kStageBytes, "the sums fit the stages");
 };
 
 struct GatedRowsParams {
     int t, inter, act;
+    int n;               // rows of x in a tile, a multiple of 16 and at most BN
     int kb_total, kb_per_split, splits;
+    int vec;             // rows of `out` start on 8-byte boundaries
     void* out;
     uint16_t* save_hi;
     uint8_t* save_lo;
@@ -559,6 +635,14 @@ __device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t adesc, uint
         : "memory");
 }
 
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_addr) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
 {
     float v;
@@ -567,7 +651,7 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
 }
 
 template <int BN, bool kBf16>
-__global__ void __launch_bounds__(GatedRowsCfg<BN>::kThreads, 2)
+__global__ void __launch_bounds__(GatedRowsCfg<BN>::kThreads, GatedRowsCfg<BN>::kBlocks)
 gated_rows_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ CUtensorMap tm_u,
     const __grid_constant__ CUtensorMap tm_x, const GatedRowsParams p)
 {
@@ -590,6 +674,8 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_constan
     int const lane = threadIdx.x & 31;
     int const tile = blockIdx.x / p.splits;
     int const rank = blockIdx.x - tile * p.splits;
+    int const row0 = blockIdx.y * p.n;
+    int const rows = min(p.n, p.t - row0);
     int const kb0 = rank * p.kb_per_split, kb1 = min(p.kb_total, kb0 + p.kb_per_split);
 
     if (threadIdx.x == 0) {
@@ -622,10 +708,10 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_constan
                     break;
                 }
                 uint32_t const fb = full_bar(stage);
-                mbar_expect_tx(fb, C::kStageBytes);
+                mbar_expect_tx(fb, C::kABytes + p.n * 128);
                 tma_load_2d(sA + stage * C::kABytes, &tm_g, fb, kb * 64, tile * 64);
                 tma_load_2d(sA + stage * C::kABytes + 8192, &tm_u, fb, kb * 64, tile * 64);
-                tma_load_2d(sB + stage * C::kBBytes, &tm_x, fb, kb * 64, 0);
+                tma_load_2d(sB + stage * C::kBBytes, &tm_x, fb, kb * 64, row0);
                 if (++stage == S) {
                     stage = 0;
                     phase ^= 1u;
@@ -635,7 +721,7 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_constan
         __syncwarp();
     } else if (warp == 1) {
         if (elect_one()) {
-            constexpr uint32_t idesc = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | ((BN >> 3) << 17) | ((128u >> 4) << 24);
+            uint32_t const idesc = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (static_cast<uint32_t>(p.n >> 3) << 17) | ((128u >> 4) << 24);
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -668,7 +754,7 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_constan
             uint32_t const t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
             for (int c = 0; c < BN; c += 16) {
-                if (c >= p.t) break;
+                if (c >= rows) break;
                 uint32_t r[16];
                 tmem_ld_32x16(t_row + c, r);
                 tmem_ld_wait();
@@ -691,31 +777,29 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_constan
     if (!failed) {
         float const* const red = reinterpret_cast<float const*>(gbase);
         uint32_t const red_addr = smem_u32(red);
-        for (int i = rank * C::kThreads + static_cast<int>(threadIdx.x); i < p.t * 64; i += C::kThreads * p.splits) {
-            int const row = i >> 6, in_tile = i & 63;
+        // four columns a thread
+        for (int i = rank * C::kThreads + static_cast<int>(threadIdx.x); i < rows * 16; i += C::kThreads * p.splits) {
+            int const row = i >> 4, in_tile = (i & 15) * 4;
             int const col = tile * 64 + in_tile;
             if (col >= p.inter) continue;
             int const at = row * C::kRedStride + in_tile;
-            float g = 0.f, u = 0.f;
-            if (p.splits == 1) {
-                g = red[at];
-                u = red[at + 64];
-            } else {
-                for (int r = 0; r < p.splits; ++r) {
+            float g[4] = {}, u[4] = {};
+            for (int r = 0; r < p.splits; ++r) {
+                float4 a, b;
+                if (p.splits == 1) {
+                    a = *reinterpret_cast<float4 const*>(red + at);
+                    b = *reinterpret_cast<float4 const*>(red + at + 64);
+                } else {
                     uint32_t const peer = map_to_cta(red_addr + 4u * at, r);
-                    g += ld_cluster_f32(peer);
-                    u += ld_cluster_f32(peer + 256u);
+                    a = ld_cluster_f32x4(peer);
+                    b = ld_cluster_f32x4(peer + 256u);
                 }
+                g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
+                u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
             }
-            if (p.save_hi != nullptr) {
-                int64_t const to = static_cast<int64_t>(row) * 2 * p.half_cols + col;
-                uint32_t const gb = to_24(g), ub = to_24(u);
-                p.save_hi[to] = static_cast<uint16_t>(gb >> 8);
-                p.save_lo[to] = static_cast<uint8_t>(gb);
-                p.save_hi[to + p.half_cols] = static_cast<uint16_t>(ub >> 8);
-                p.save_lo[to + p.half_cols] = static_cast<uint8_t>(ub);
-            }
-            store16<kBf16>(p.out, static_cast<int64_t>(row) * p.inter + col, gate_value(g, p.act) * u);
+            int64_t const out_row = row0 + row;
+            finish_four<kBf16>(g, u, p.act, p.save_hi, p.save_lo, out_row * 2 * p.half_cols + col, p.half_cols, p.out,
+                out_row * p.inter + col, p.inter - col, p.vec != 0);
         }
     }
     __syncwarp();
@@ -770,29 +854,8 @@ __global__ void gated16_finish_kernel(float const* __restrict__ ws, int splits, 
         g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
         u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
     }
-    if (save_hi != nullptr) {
-        int64_t const at = row * 2 * half_cols + col;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint32_t b[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = to_24(h ? u[j] : g[j]);
-            *reinterpret_cast<uint2*>(save_hi + at + h * half_cols) =
-                make_uint2((b[0] >> 8) | ((b[1] >> 8) << 16), (b[2] >> 8) | ((b[3] >> 8) << 16));
-            *reinterpret_cast<uint32_t*>(save_lo + at + h * half_cols) =
-                (b[0] & 0xFFu) | ((b[1] & 0xFFu) << 8) | ((b[2] & 0xFFu) << 16) | (b[3] << 24);
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = gate_value(g[j], act) * u[j];
-    if (vec && col + 4 <= cols) {
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + row * cols + col) =
-            make_uint2(pack16<kBf16>(g[0], g[1]), pack16<kBf16>(g[2], g[3]));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (col + j < cols) store16<kBf16>(out, row * cols + col + j, g[j]);
-    }
+    finish_four<kBf16>(g, u, act, save_hi, save_lo, row * 2 * half_cols + col, half_cols, out, row * cols + col, cols - col,
+        vec != 0);
 }
 
 // ------------------------------------------------------------------------------------------------ dg and du
@@ -875,27 +938,66 @@ inline int make_map16(CUtensorMap* map, const void* base, int64_t rows, int64_t 
 
 inline int64_t gated_half_cols(int64_t inter) { return (inter + 15) / 16 * 16; }
 
-constexpr int kGatedRowsMax = 128;      // rows of x up to which the few-rows kernel runs the forward pass
-
 // Tiles and slices of the products. Pure host arithmetic.
 struct Gated16Plan {
+    int rows_n;          // forward: rows of x in a tile of the few-rows kernel, or 0 for the pair kernel
     int tiles_m, tiles_n, kb, kb_half, splits, kb_per_split;
     int64_t ws_bytes, ws_cols;
 };
 
 inline int tiles_of(int64_t n, int64_t w) { return static_cast<int>((n + w - 1) / w); }
 
+// FSO_B200_GATED=pair | rows keeps the forward pass of more than 128 rows on one of its two kernels (measurement; read once).
+inline int forced_gated_kernel()
+{
+    static int const v = [] {
+        const char* e = std::getenv("FSO_B200_GATED");
+        return e == nullptr ? 0 : std::strcmp(e, "pair") == 0 ? 1 : std::strcmp(e, "rows") == 0 ? 2 : 0;
+    }();
+    return v;
+}
+
+// The forward pass. Both kernels are costed in microseconds of a B200, with constants fitted to sweeps over 129 to 2900 rows
+// on five weights with either kernel forced: rounds of the schedule times the blocks of a slice (a 64-wide block is 512 cycles
+// at 1.55 GHz for 256 rows of x, in proportion below, 264 cycles at the least), what a tile costs beside them, and for the
+// pair kernel the traffic of split sums through L2.
 inline Gated16Plan plan_gated16_forward(int64_t t, int64_t k, int64_t inter, int sms)
 {
     Gated16Plan p{};
-    if (t <= kGatedRowsMax) return p;      // no workspace
+    p.kb = tiles_of(k, 64);
+    int const pairs = std::max(1, sms / 2);
+    // few rows: token tiles of at most 256, equal, multiples of 16
+    int const row_tiles = tiles_of(t, 256), weight_tiles = tiles_of(inter, 64);
+    int const n = static_cast<int>((tiles_of(t, row_tiles) + 15) / 16 * 16);
+    int64_t const tiles = static_cast<int64_t>(row_tiles) * weight_tiles;
+    int const slots = n <= 128 ? 2 * sms : sms;
+    // slices: as many as all SMs need to have work, at most eight (the portable cluster size), of at least four blocks, none
+    // empty
+    int s = 1;
+    while (s < 8 && tiles * s * 2 <= (n <= 128 ? 3 * sms : sms) && (s + 1) * 4 <= p.kb) ++s;
+    int const per = tiles_of(p.kb, s);
+    double const rows_us = std::ceil(static_cast<double>(tiles * s) / slots) * (per * std::max(264, 2 * n) / 1550.0 * (n <= 128 ? 2 : 1)
+        + 2.0 + 0.035 * n) + 3.0;
+    // pairs
     p.tiles_m = tiles_of(t, 256);
     p.tiles_n = tiles_of(inter, 128);
-    p.kb = tiles_of(k, 64);
     p.ws_cols = 2 * gated_half_cols(inter);
-    // slices of the contraction where the tiles would leave half of the SM pairs without work
-    pick_splits(static_cast<int64_t>(p.tiles_m) * p.tiles_n, p.kb, sms / 2, 8, 16, &p.splits, &p.kb_per_split);
-    p.ws_bytes = p.splits > 1 ? p.splits * t * p.ws_cols * 4 : 0;
+    double pair_us = 1e30;
+    int pair_s = 1;
+    for (int q = 1; q <= 16 && (q == 1 || q * 4 <= p.kb); ++q) {
+        double const rounds = std::ceil(static_cast<double>(p.tiles_m) * p.tiles_n * q / pairs);
+        double const us = rounds * tiles_of(p.kb, q) * (512 / 1550.0) + 9.0
+            + (q > 1 ? 3.0 + static_cast<double>(q) * t * p.ws_cols * 8 / 8e6 : 0.0);
+        if (us < pair_us) {
+            pair_us = us;
+            pair_s = q;
+        }
+    }
+    bool const rows = t <= 128 || (forced_gated_kernel() == 0 ? rows_us < pair_us : forced_gated_kernel() == 2);
+    p.rows_n = rows ? n : 0;
+    p.kb_per_split = rows ? per : tiles_of(p.kb, pair_s);
+    p.splits = tiles_of(p.kb, p.kb_per_split);
+    p.ws_bytes = !rows && p.splits > 1 ? p.splits * t * p.ws_cols * 4 : 0;
     return p;
 }
 
@@ -975,17 +1077,6 @@ inline void fill_product(Gated16Product& q, Gated16Plan const& pl)
 
 inline unsigned blocks_for(int64_t threads, int per_block) { return static_cast<unsigned>((threads + per_block - 1) / per_block); }
 
-// Slices of the contraction for `tiles` CTAs' worth of rows: as many as all SMs need to have work (two CTAs fit), at most
-// eight (the portable cluster size), at least four 64-wide blocks in each and none empty.
-inline void gated_rows_slices(int64_t tiles, int kb, int sms, GatedRowsParams& p)
-{
-    int s = 1;
-    while (s < 8 && tiles * s * 2 <= 3 * sms && (s + 1) * 4 <= kb) ++s;
-    p.kb_total = kb;
-    p.kb_per_split = (kb + s - 1) / s;
-    p.splits = (kb + p.kb_per_split - 1) / p.kb_per_split;
-}
-
 template <int BN, bool kBf16>
 inline int launch_gated_rows(const void* x, int64_t ldx, const void* gate_up, int64_t k, GatedRowsParams p, cudaStream_t stream)
 {
@@ -998,12 +1089,11 @@ inline int launch_gated_rows(const void* x, int64_t ldx, const void* gate_up, in
     CUtensorMap mg, mu, mx;
     rc = make_map16(&mg, w, p.inter, k, k, 64);
     if (rc == 0) rc = make_map16(&mu, w + p.inter * k, p.inter, k, k, 64);
-    if (rc == 0) rc = make_map16(&mx, x, p.t, k, ldx, BN);
+    if (rc == 0) rc = make_map16(&mx, x, p.t, k, ldx, p.n);
     if (rc != 0) return rc;
-    int const tiles = (p.inter + 63) / 64;
-    gated_rows_slices(tiles, static_cast<int>((k + 63) / 64), sm_count(), p);
+    int const tiles = (p.inter + 63) / 64, row_tiles = (p.t + p.n - 1) / p.n;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.splits), 1, 1);
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.splits), static_cast<unsigned>(row_tiles), 1);
     cfg.blockDim = dim3(C::kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmemBytes;
     cfg.stream = stream;
@@ -1022,22 +1112,28 @@ template <bool kBf16>
 inline int gated_forward(const void* x, int64_t ldx, const void* gate_up, void* h, void* save_hi, void* save_lo, int64_t t,
     int64_t k, int64_t inter, int act, void* ws, cudaStream_t stream)
 {
-    if (t <= kGatedRowsMax) {
+    int const sms = sm_count();
+    Gated16Plan const pl = plan_gated16_forward(t, k, inter, sms);
+    if (pl.rows_n > 0) {
         GatedRowsParams r{};
         r.t = static_cast<int>(t);
         r.inter = static_cast<int>(inter);
         r.act = act;
+        r.n = pl.rows_n;
+        r.kb_total = pl.kb;
+        r.kb_per_split = pl.kb_per_split;
+        r.splits = pl.splits;
         r.out = h;
+        r.vec = inter % 4 == 0 && (reinterpret_cast<uintptr_t>(h) & 7u) == 0;
         r.save_hi = static_cast<uint16_t*>(save_hi);
         r.save_lo = static_cast<uint8_t*>(save_lo);
         r.half_cols = gated_half_cols(inter);
-        return t <= 16 ? launch_gated_rows<16, kBf16>(x, ldx, gate_up, k, r, stream)
-            : t <= 32  ? launch_gated_rows<32, kBf16>(x, ldx, gate_up, k, r, stream)
-            : t <= 64  ? launch_gated_rows<64, kBf16>(x, ldx, gate_up, k, r, stream)
-                       : launch_gated_rows<128, kBf16>(x, ldx, gate_up, k, r, stream);
+        return r.n <= 16 ? launch_gated_rows<16, kBf16>(x, ldx, gate_up, k, r, stream)
+            : r.n <= 32  ? launch_gated_rows<32, kBf16>(x, ldx, gate_up, k, r, stream)
+            : r.n <= 64  ? launch_gated_rows<64, kBf16>(x, ldx, gate_up, k, r, stream)
+            : r.n <= 128 ? launch_gated_rows<128, kBf16>(x, ldx, gate_up, k, r, stream)
+                         : launch_gated_rows<256, kBf16>(x, ldx, gate_up, k, r, stream);
     }
-    int const sms = sm_count();
-    Gated16Plan const pl = plan_gated16_forward(t, k, inter, sms);
     CUtensorMap m[5];
     uint16_t const* const w = static_cast<uint16_t const*>(gate_up);
     int rc = make_map16(&m[0], x, t, k, ldx, 128);
