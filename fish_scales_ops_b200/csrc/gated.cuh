@@ -58,7 +58,6 @@ struct Gated16Product {
 struct Gated16Params {
     Gated16Product first, second;      // forward: first alone; backward: in either order, tiles_m = 0 where one is not wanted
     int first_is_dw;
-    int act;
     uint16_t* save_hi;   // forward: upper 16 of the 24 bits kept of g and u, [rows, 2 * half_cols], or nullptr
     uint8_t* save_lo;    // forward: lower 8 bits
     int64_t half_cols;   // columns from g to u in the saved arrays and in split sums
@@ -76,25 +75,33 @@ __device__ __forceinline__ float logistic(float v) { return __fdividef(1.f, 1.f 
 constexpr float kGeluC = 0.79788456080286535588f;      // sqrt(2 / pi)
 constexpr float kGeluCubic = 0.044715f;
 
-__device__ __forceinline__ float gate_value(float g, int act)
+template <int ACT>
+__device__ __forceinline__ float gate_value_of(float g)
 {
-    if (act == FSO_ACT_SILU) return g * logistic(g);
-    if (act == FSO_ACT_GELU) return g * normcdff(g);
-    return g * logistic(2.f * kGeluC * (g + kGeluCubic * g * g * g));
+    if constexpr (ACT == FSO_ACT_SILU) return g * logistic(g);
+    else if constexpr (ACT == FSO_ACT_GELU) return g * normcdff(g);
+    else return g * logistic(2.f * kGeluC * (g + kGeluCubic * g * g * g));
 }
 
-__device__ __forceinline__ void gate_value_slope(float g, int act, float& a, float& s)
+__device__ __forceinline__ float gate_value(float g, int act)
+{
+    if (act == FSO_ACT_SILU) return gate_value_of<FSO_ACT_SILU>(g);
+    if (act == FSO_ACT_GELU) return gate_value_of<FSO_ACT_GELU>(g);
+    return gate_value_of<FSO_ACT_GELU_TANH>(g);
+}
+
+template <int ACT>
+__device__ __forceinline__ void gate_value_slope(float g, float& a, float& s)
 {
     float p, dp;      // dp = g P'(g)
-    if (act == FSO_ACT_SILU) {
+    if constexpr (ACT == FSO_ACT_SILU) {
         p = logistic(g);
         dp = g * p * (1.f - p);
-    } else if (act == FSO_ACT_GELU) {
+    } else if constexpr (ACT == FSO_ACT_GELU) {
         p = normcdff(g);
         dp = g * 0.39894228040143267794f * __expf(-0.5f * g * g);
     } else {
-        float const z2 = 2.f * kGeluC * (g + kGeluCubic * g * g * g);
-        p = logistic(z2);
+        p = logistic(2.f * kGeluC * (g + kGeluCubic * g * g * g));
         dp = g * p * (1.f - p) * 2.f * kGeluC * (1.f + 3.f * kGeluCubic * g * g);
     }
     a = g * p;
@@ -251,7 +258,9 @@ __device__ __forceinline__ void tc_mma_f16_pair(uint32_t d_tmem, uint64_t adesc,
 // MMAs. Forward: CTA 0 stages 128 rows of G, CTA 1 the same 128 rows of U, so a CTA's accumulator holds g in columns
 // 0..127 and u in columns 128..255 of its own 128 tokens.
 // Maps: forward x, G, U (boxes of 128 rows); backward x, G, U, dg, du (boxes of 64 rows).
-template <int MODE, bool kBf16>
+// ACT: the activation of the forward pass (kernels of their own: with the three of them in one epilogue its code no longer
+// fits the instruction cache beside the main loop; 1500 rows on 1032 x 2744 take 33 us that way).
+template <int MODE, bool kBf16, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Gated16Cfg::kThreads, 1)
 gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_g,
     const __grid_constant__ CUtensorMap tm_u, const __grid_constant__ CUtensorMap tm_dg, const __grid_constant__ CUtensorMap tm_du,
@@ -515,7 +524,7 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                         });
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) g[i] = gate_value(g[i], p.act) * u[i];
+                    for (int i = 0; i < 32; ++i) g[i] = gate_value_of<ACT>(g[i]) * u[i];
                     if (q.vec) {
                         uint16_t* const to = static_cast<uint16_t*>(q.out) + static_cast<int64_t>(row0) * q.ldo + col;
 #pragma unroll
@@ -863,9 +872,9 @@ __global__ void gated16_finish_kernel(float const* __restrict__ ws, int splits, 
 // dg = dh * u * act'(g), du = dh * act(g) from the saved g and u, rounded to the 16 bits in which the tensor cores take
 // them (the one rounding of the backward pass before its products). Bound by memory: 2 + 2 * 3 bytes in and 4 out for
 // each element. Eight columns a thread.
-template <bool kBf16>
-__global__ void gated_slopes_kernel(const void* __restrict__ dh, int64_t ldh, int dh_vec, uint16_t const* __restrict__ save_hi,
-    uint8_t const* __restrict__ save_lo, int rows, int cols, int64_t half_cols, int act, uint16_t* __restrict__ out)
+template <bool kBf16, int ACT>
+__global__ void __launch_bounds__(256) gated_slopes_kernel(const void* __restrict__ dh, int64_t ldh, int dh_vec, uint16_t const* __restrict__ save_hi,
+    uint8_t const* __restrict__ save_lo, int rows, int cols, int64_t half_cols, uint16_t* __restrict__ out)
 {
     griddep_launch_dependents();
     griddep_wait();
@@ -900,7 +909,7 @@ __global__ void gated_slopes_kernel(const void* __restrict__ dh, int64_t ldh, in
         float const g = from_24((ghw[j / 2] >> (16 * (j & 1))) & 0xFFFFu, (glw[j / 4] >> (8 * (j & 3))) & 0xFFu);
         float const u = from_24((uhw[j / 2] >> (16 * (j & 1))) & 0xFFFFu, (ulw[j / 4] >> (8 * (j & 3))) & 0xFFu);
         float a, s;
-        gate_value_slope(g, act, a, s);
+        gate_value_slope<ACT>(g, a, s);
         dg[j] = d[j] * u * s;
         du[j] = d[j] * a;
     }
@@ -1048,11 +1057,11 @@ inline int launch_chained(const char* what, void (*kernel)(Params...), unsigned 
     return launch_status(what);
 }
 
-template <int MODE, bool kBf16>
+template <int MODE, bool kBf16, int ACT>
 inline int launch_gated16(CUtensorMap const (&m)[5], Gated16Params const& p, int sms, cudaStream_t stream)
 {
     static std::atomic<uint64_t> done{0};
-    auto kernel = gated16_pair_kernel<MODE, kBf16>;
+    auto kernel = gated16_pair_kernel<MODE, kBf16, ACT>;
     int const rc = ensure_smem_attr(kernel, Gated16Cfg::kSmemBytes, done);
     if (rc != 0) return rc;
     int64_t const items = static_cast<int64_t>(p.first.tiles_m) * p.first.tiles_n * p.first.splits
@@ -1149,11 +1158,12 @@ inline int gated_forward(const void* x, int64_t ldx, const void* gate_up, void* 
     p.first.out = h;
     p.first.ldo = inter;
     p.first.ws = pl.splits > 1 ? static_cast<float*>(ws) : nullptr;
-    p.act = act;
     p.save_hi = static_cast<uint16_t*>(save_hi);
     p.save_lo = static_cast<uint8_t*>(save_lo);
     p.half_cols = gated_half_cols(inter);
-    rc = launch_gated16<G16_FORWARD, kBf16>(m, p, sms, stream);
+    rc = act == FSO_ACT_SILU ? launch_gated16<G16_FORWARD, kBf16, FSO_ACT_SILU>(m, p, sms, stream)
+        : act == FSO_ACT_GELU ? launch_gated16<G16_FORWARD, kBf16, FSO_ACT_GELU>(m, p, sms, stream)
+                              : launch_gated16<G16_FORWARD, kBf16, FSO_ACT_GELU_TANH>(m, p, sms, stream);
     if (rc != 0 || pl.splits == 1) return rc;
     return launch_chained("gated16_finish_kernel", gated16_finish_kernel<kBf16>, blocks_for(t * (p.half_cols / 4), 128), 128, 0,
         stream, p.first.ws, pl.splits, p.first.rows, p.first.cols, p.half_cols, act, p.save_hi, p.save_lo, h, p.first.vec);
@@ -1183,9 +1193,11 @@ inline int gated_backward(const void* dh, int64_t ldh, const void* x, int64_t ld
     int64_t const hc = gated_half_cols(inter);
     uint16_t* const slopes = static_cast<uint16_t*>(ws);
     int const dh_vec = inter % 8 == 0 && ldh % 8 == 0 && aligned16(dh);
-    int rc = launch_chained("gated_slopes_kernel", gated_slopes_kernel<kBf16>, blocks_for(t * (hc / 8), 256), 256, 0, stream, dh, ldh,
+    auto slopes_kernel = act == FSO_ACT_SILU ? gated_slopes_kernel<kBf16, FSO_ACT_SILU>
+        : act == FSO_ACT_GELU ? gated_slopes_kernel<kBf16, FSO_ACT_GELU> : gated_slopes_kernel<kBf16, FSO_ACT_GELU_TANH>;
+    int rc = launch_chained("gated_slopes_kernel", slopes_kernel, blocks_for(t * (hc / 8), 256), 256, 0, stream, dh, ldh,
         dh_vec, static_cast<uint16_t const*>(save_hi), static_cast<uint8_t const*>(save_lo), static_cast<int>(t),
-        static_cast<int>(inter), hc, act, slopes);
+        static_cast<int>(inter), hc, slopes);
     if (rc != 0) return rc;
 
     Gated16Plan px, pw;
@@ -1219,7 +1231,7 @@ inline int gated_backward(const void* dh, int64_t ldh, const void* x, int64_t ld
     qw.ldo = k;
     qw.out_half = inter * k;
     qw.ws = pw.splits > 1 ? sums_w : nullptr;
-    rc = launch_gated16<G16_BACKWARD, kBf16>(m, p, sms, stream);
+    rc = launch_gated16<G16_BACKWARD, kBf16, 0>(m, p, sms, stream);
     if (rc == 0 && dx != nullptr && px.splits > 1)
         rc = launch_chained("gated16_sum_kernel", gated16_sum_kernel<kBf16>, blocks_for(t * (k / 8), 256), 256, 0, stream, sums_x,
             px.splits, t * px.ws_cols, t, static_cast<int>(k), px.ws_cols, static_cast<uint16_t*>(dx), k);
