@@ -366,30 +366,38 @@ def _gated_ws_bytes(query: str, t: int, k: int, inter: int, dev: int) -> int:
     return _GATED_WS[key]
 
 
+def gated_saved_cols(inter: int) -> int:
+    """Bytes that a row of the saved projections takes: 24 bits for each of its 2 * INTER values, padded to 16 columns."""
+    return 6 * _align(inter, 16)
+
+
+def _saved_parts(saved, t: int, inter: int):
+    """Addresses of the upper 16 and of the lower 8 bits in the one buffer of the saved projections."""
+    p = saved.data_ptr()
+    return p, p + 4 * t * _align(inter, 16)
+
+
 def gated_linear(x, gate_up, activation: int, save: bool):
-    """x [T, K], gate_up [2I, K] -> (h [T, I], saved upper 16 bits, saved lower 8 bits); the saved arrays are None
-    without ``save``."""
+    """x [T, K], gate_up [2I, K] -> (h [T, I], saved projections as uint8 [T, gated_saved_cols(I)], None without
+    ``save``)."""
     t, k = x.shape
     inter = gate_up.shape[0] // 2
     h = x.new_empty((t, inter))
-    hi = lo = None
-    if save:
-        cols = 2 * _align(inter, 16)
-        hi, lo = x.new_empty((t, cols), dtype=torch.int16), x.new_empty((t, cols), dtype=torch.uint8)
+    saved = x.new_empty((t, gated_saved_cols(inter)), dtype=torch.uint8) if save else None
     if t > 0:
         x, ldx = rows_in_place(x)
         with on_device(x.device):
             need = _gated_ws_bytes("fso_gated_linear_ws_bytes", t, k, inter, x.get_device())
             ws = x.new_empty((need,), dtype=torch.uint8) if need else None
-            rc = call_on(x, lib().fso_gated_linear, x.data_ptr(), ldx, gate_up.data_ptr(), h.data_ptr(),
-                         hi.data_ptr() if save else None, lo.data_ptr() if save else None, t, k, inter, DTYPES_16[x.dtype],
-                         activation, None if ws is None else ws.data_ptr(), need)
+            hi, lo = _saved_parts(saved, t, inter) if save else (None, None)
+            rc = call_on(x, lib().fso_gated_linear, x.data_ptr(), ldx, gate_up.data_ptr(), h.data_ptr(), hi, lo, t, k, inter,
+                         DTYPES_16[x.dtype], activation, None if ws is None else ws.data_ptr(), need)
         if rc != 0:
             check(rc, "fso_gated_linear")
-    return h, hi, lo
+    return h, saved
 
 
-def gated_linear_backward(dh, x, gate_up, hi, lo, activation: int, need_x: bool, need_w: bool):
+def gated_linear_backward(dh, x, gate_up, saved, activation: int, need_x: bool, need_w: bool):
     """(dx [T, K] or empty, dgate_up [2I, K] or empty) for dh [T, I]."""
     t, k = x.shape
     inter = gate_up.shape[0] // 2
@@ -402,9 +410,10 @@ def gated_linear_backward(dh, x, gate_up, hi, lo, activation: int, need_x: bool,
         with on_device(x.device):
             need = _gated_ws_bytes("fso_gated_linear_backward_ws_bytes", t, k, inter, x.get_device())
             ws = x.new_empty((need,), dtype=torch.uint8)
+            hi, lo = _saved_parts(saved, t, inter)
             rc = call_on(x, lib().fso_gated_linear_backward, dh.data_ptr(), dh.stride(0) if t > 1 else inter, x.data_ptr(), ldx,
-                         gate_up.data_ptr(), hi.data_ptr(), lo.data_ptr(), dx.data_ptr() if need_x else None,
-                         dw.data_ptr() if need_w else None, t, k, inter, DTYPES_16[x.dtype], activation, ws.data_ptr(), need)
+                         gate_up.data_ptr(), hi, lo, dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None, t, k,
+                         inter, DTYPES_16[x.dtype], activation, ws.data_ptr(), need)
         if rc != 0:
             check(rc, "fso_gated_linear_backward")
     return dx, dw

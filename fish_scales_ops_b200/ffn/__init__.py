@@ -52,49 +52,45 @@ def _refuse(op: str, why: str):
 
 def _gated_linear_body(x, gate_up, activation, save):
     _check("fish_scales_ops::gated_linear", x, gate_up, activation)
-    h, hi, lo = _ops.gated_linear(x, gate_up, _ops.GATE_ACTIVATIONS[activation], save)
-    if not save:
-        hi, lo = (x.new_empty((x.shape[0], 0), dtype=d) for d in (torch.int16, torch.uint8))
-    return h, hi, lo
+    h, saved = _ops.gated_linear(x, gate_up, _ops.GATE_ACTIVATIONS[activation], save)
+    return h, saved if save else x.new_empty((x.shape[0], 0), dtype=torch.uint8)
 
 
-def _gated_linear_backward_body(dh, x, gate_up, saved_hi, saved_lo, activation, need_x, need_w):
+def _gated_linear_backward_body(dh, x, gate_up, saved, activation, need_x, need_w):
     op = "fish_scales_ops::gated_linear_backward"
     _check(op, x, gate_up, activation)
     t, inter = int(x.shape[0]), int(gate_up.shape[0]) // 2
-    cols = 2 * _ops._align(inter, 16)
+    cols = _ops.gated_saved_cols(inter)
     if tuple(dh.shape) != (t, inter) or dh.dtype != x.dtype or dh.device != x.device:
         _refuse(op, f"dh must be {x.dtype} [{t}, {inter}] on {x.device}, got {dh.dtype} {tuple(dh.shape)} on {dh.device}")
-    for s, dtype in ((saved_hi, torch.int16), (saved_lo, torch.uint8)):
-        if tuple(s.shape) != (t, cols) or s.dtype != dtype or s.device != x.device or not s.is_contiguous():
-            _refuse(op, f"the saved arrays must be the int16 and the uint8 [{t}, {cols}] that fish_scales_ops::gated_linear "
-                        f"returned with save, got {s.dtype} {tuple(s.shape)}")
-    return _ops.gated_linear_backward(dh, x, gate_up, saved_hi, saved_lo, _ops.GATE_ACTIVATIONS[activation], need_x, need_w)
+    if tuple(saved.shape) != (t, cols) or saved.dtype != torch.uint8 or saved.device != x.device or not saved.is_contiguous():
+        _refuse(op, f"saved must be the uint8 [{t}, {cols}] that fish_scales_ops::gated_linear returned with save, got "
+                    f"{saved.dtype} {tuple(saved.shape)}")
+    return _ops.gated_linear_backward(dh, x, gate_up, saved, _ops.GATE_ACTIVATIONS[activation], need_x, need_w)
 
 
 _gated_linear_op = torch.library.custom_op(
     "fish_scales_ops::gated_linear",
     mutates_args=(),
-    schema="(Tensor x, Tensor gate_up, str activation, bool save) -> (Tensor, Tensor, Tensor)",
+    schema="(Tensor x, Tensor gate_up, str activation, bool save) -> (Tensor, Tensor)",
 )(_gated_linear_body)
 
 _gated_linear_backward_op = torch.library.custom_op(
     "fish_scales_ops::gated_linear_backward",
     mutates_args=(),
-    schema="(Tensor dh, Tensor x, Tensor gate_up, Tensor saved_hi, Tensor saved_lo, str activation, bool need_x, "
-           "bool need_w) -> (Tensor, Tensor)",
+    schema="(Tensor dh, Tensor x, Tensor gate_up, Tensor saved, str activation, bool need_x, bool need_w) "
+           "-> (Tensor, Tensor)",
 )(_gated_linear_backward_body)
 
 
 @_gated_linear_op.register_fake
 def _gated_linear_fake(x, gate_up, activation, save):
     t, inter = x.shape[0], gate_up.shape[0] // 2
-    cols = 2 * ((inter + 15) // 16 * 16) if save else 0
-    return (x.new_empty((t, inter)), x.new_empty((t, cols), dtype=torch.int16), x.new_empty((t, cols), dtype=torch.uint8))
+    return x.new_empty((t, inter)), x.new_empty((t, 6 * ((inter + 15) // 16 * 16) if save else 0), dtype=torch.uint8)
 
 
 @_gated_linear_backward_op.register_fake
-def _gated_linear_backward_fake(dh, x, gate_up, saved_hi, saved_lo, activation, need_x, need_w):
+def _gated_linear_backward_fake(dh, x, gate_up, saved, activation, need_x, need_w):
     return (x.new_empty((x.shape[0] if need_x else 0, x.shape[1])),
             x.new_empty((gate_up.shape[0] if need_w else 0, x.shape[1])))
 
@@ -102,19 +98,19 @@ def _gated_linear_backward_fake(dh, x, gate_up, saved_hi, saved_lo, activation, 
 def _setup_context(ctx, inputs, output):
     x, gate_up, activation, save = inputs
     if not save:
-        raise RuntimeError("fish_scales_ops::gated_linear: a gradient needs the arrays that save=True keeps")
-    ctx.save_for_backward(x, gate_up, output[1], output[2])
+        raise RuntimeError("fish_scales_ops::gated_linear: a gradient needs what save=True keeps")
+    ctx.save_for_backward(x, gate_up, output[1])
     ctx.activation = activation
-    ctx.mark_non_differentiable(output[1], output[2])
+    ctx.mark_non_differentiable(output[1])
     ctx.set_materialize_grads(False)
 
 
 def _gradients(backward, ctx, dh):
-    x, gate_up, hi, lo = ctx.saved_tensors
+    x, gate_up, saved = ctx.saved_tensors
     need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
     if dh is None or not (need_x or need_w):
         return None, None
-    dx, dw = backward(dh, x, gate_up, hi, lo, ctx.activation, need_x, need_w)
+    dx, dw = backward(dh, x, gate_up, saved, ctx.activation, need_x, need_w)
     return dx if need_x else None, dw if need_w else None
 
 
@@ -132,8 +128,8 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_up, activation):
         _check("fso.ffn.gated_linear", x, gate_up, activation)
-        h, hi, lo = _ops.gated_linear(x, gate_up, _ops.GATE_ACTIVATIONS[activation], True)
-        ctx.save_for_backward(x, gate_up, hi, lo)
+        h, saved = _ops.gated_linear(x, gate_up, _ops.GATE_ACTIVATIONS[activation], True)
+        ctx.save_for_backward(x, gate_up, saved)
         ctx.activation = activation
         return h
 
@@ -149,8 +145,8 @@ def _differentiable_once(ctx, dh):
     return (*_gradients(_eager_backward, ctx, dh), None)
 
 
-def _eager_backward(dh, x, gate_up, hi, lo, activation, need_x, need_w):
-    return _ops.gated_linear_backward(dh, x, gate_up, hi, lo, _ops.GATE_ACTIVATIONS[activation], need_x, need_w)
+def _eager_backward(dh, x, gate_up, saved, activation, need_x, need_w):
+    return _ops.gated_linear_backward(dh, x, gate_up, saved, _ops.GATE_ACTIVATIONS[activation], need_x, need_w)
 
 
 # ------------------------------------------------------------------------------------------------ public functions

@@ -68,9 +68,9 @@ def test_exported_names(fso):
                                      "gated_linear"}
     assert fso.ffn.ACTIVATIONS == fso.int4.ACTIVATIONS == ("silu", "gelu", "gelu_tanh")
     for name, want in {
-        "gated_linear": "(Tensor x, Tensor gate_up, str activation, bool save) -> (Tensor, Tensor, Tensor)",
-        "gated_linear_backward": "(Tensor dh, Tensor x, Tensor gate_up, Tensor saved_hi, Tensor saved_lo, str activation, "
-                                 "bool need_x, bool need_w) -> (Tensor, Tensor)",
+        "gated_linear": "(Tensor x, Tensor gate_up, str activation, bool save) -> (Tensor, Tensor)",
+        "gated_linear_backward": "(Tensor dh, Tensor x, Tensor gate_up, Tensor saved, str activation, bool need_x, "
+                                 "bool need_w) -> (Tensor, Tensor)",
         "int4_linear": "(Tensor x, Tensor codes, Tensor scale, Tensor? zero=None, Tensor? bias=None) -> Tensor",
         "int4_gated_linear": "(Tensor x, Tensor codes, Tensor scale, Tensor? zero, str activation) -> Tensor",
     }.items():
