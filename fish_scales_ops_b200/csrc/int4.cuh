@@ -74,6 +74,27 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t saddr, uint32_t (&r)[4])
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(saddr) : "memory");
 }
 
+__device__ __forceinline__ uint32_t lds_u16(uint32_t saddr)
+{
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(saddr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ uint32_t lds_u8(uint32_t saddr)
+{
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(saddr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ uint4 lds_v4(uint32_t saddr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(saddr) : "memory");
+    return v;
+}
+
 template <int NT>
 struct Int4Cfg {
     static constexpr int kRT = 2;                // 16-row tiles of a warp
@@ -211,23 +232,17 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
         // scales and zero points of a row and group: lane (g, t) needs those of rows g and g + 8 of each 16
         uint32_t const scale_width = p.scale_type == 2 ? 4 : 2;
         int const group0 = (kq * 128) >> p.group_shift;      // of this warp inside a stage (0 where a group spans stages)
+        // (no branch on the kinds of scale and zero point: a stage stays one block of instructions, whose loads the compiler
+        // moves ahead of the products)
         auto scale_of = [&](uint32_t sbase, int row, int j) -> float {      // row 0..63 of the tile
             uint32_t const at = sbase + C::kScaleOff + (row >> 5) * 2048 + ((group0 + j) * 32 + (row & 31)) * scale_width;
-            if (p.scale_type == 2) {
-                float v;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-                return v;
-            }
-            uint16_t v;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
-            return p.scale_type == 0 ? __uint_as_float(static_cast<uint32_t>(v) << 16) : __half2float(__ushort_as_half(v));
+            uint32_t const upper = lds_u16(at + scale_width - 2), lower = lds_u16(at);
+            return p.scale_type == 1 ? __half2float(__ushort_as_half(static_cast<uint16_t>(upper)))
+                                     : __uint_as_float(upper << 16 | (p.scale_type == 2 ? lower : 0u));
         };
         auto zero_of = [&](uint32_t sbase, int row, int j) -> uint32_t {
-            uint32_t z = 8;
-            if (p.has_zero)
-                asm volatile("ld.shared.u8 %0, [%1];"
-                             : "=r"(z) : "r"(sbase + C::kZeroOff + (row >> 5) * 512 + (group0 + j) * 32 + (row & 31)) : "memory");
-            return ((kBf16 ? 0x4300u : 0x6400u) + z) * 0x10001u;
+            uint32_t const z = lds_u8(sbase + C::kZeroOff + (row >> 5) * 512 + (group0 + j) * 32 + (row & 31));
+            return ((kBf16 ? 0x4300u : 0x6400u) + (p.has_zero ? z : 8u)) * 0x10001u;
         };
         int stage = 0;
         uint32_t phase = 0;
@@ -258,11 +273,7 @@ int4_rows_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constan
                     uint32_t bx[NT][4];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        uint4 v;
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                     : "r"(sbase + (c & 1 ? xoff1 : xoff0) + (c >> 1) * 1024 * NT + n * 1024)
-                                     : "memory");
+                        uint4 const v = lds_v4(sbase + (c & 1 ? xoff1 : xoff0) + (c >> 1) * 1024 * NT + n * 1024);
                         bx[n][0] = __byte_perm(v.x, v.z, 0x5410);      // elements 0 and 4
                         bx[n][1] = __byte_perm(v.x, v.z, 0x7632);      // 1 and 5
                         bx[n][2] = __byte_perm(v.y, v.w, 0x5410);      // 2 and 6
