@@ -56,6 +56,7 @@ SIGNATURES = {
     "fso_gated_linear": [_c_p, _c_i64] + [_c_p] * 4 + [_c_i64] * 5 + [_c_p, _c_i64, _c_p],
     "fso_gated_linear_backward_ws_bytes": [_c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64)],
     "fso_gated_linear_backward": [_c_p, _c_i64, _c_p, _c_i64] + [_c_p] * 5 + [_c_i64] * 5 + [_c_p, _c_i64, _c_p],
+    "fso_int4_pack_codes": [_c_p, _c_p, _c_i64, _c_i64, _c_p],
     "fso_int4_quantize": [_c_p] * 4 + [_c_i64] * 5 + [_c_p],
     "fso_int4_linear": [_c_p, _c_i64] + [_c_p] * 5 + [_c_i64] * 6 + [_c_p],
     "fso_int4_gated_linear": [_c_p, _c_i64] + [_c_p] * 4 + [_c_i64] * 7 + [_c_p],

@@ -424,6 +424,14 @@ def int4_half_cols(rows: int) -> int:
     return _align((rows + 1) // 2, 16)
 
 
+def int4_pack_codes(codes: torch.Tensor) -> torch.Tensor:
+    """uint8 [N, K/2] as checkpoints store them -> the order in which the kernels read them."""
+    n, k = int(codes.shape[0]), 2 * int(codes.shape[1])
+    packed = torch.empty_like(codes)
+    check(call_on(codes, lib().fso_int4_pack_codes, codes.data_ptr(), packed.data_ptr(), n, k), "fso_int4_pack_codes")
+    return packed
+
+
 def int4_linear(x, codes, scale, zero, bias):
     """x [M, K] and a 4-bit weight of N rows (scale and zero [K/group, 2 * half]) -> y [M, N]."""
     m, k = x.shape

@@ -760,7 +760,7 @@ static int check_int4(const char* op, int64_t m, int64_t rows, int64_t k, int64_
     FSO_REQUIRE(group >= 32 && (group & (group - 1)) == 0 && k % group == 0,
         "%s: the group size %lld must be a power of two of at least 32 that divides K = %lld", op, static_cast<long long>(group),
         static_cast<long long>(k));
-    FSO_REQUIRE(m <= 65535 * 8 && rows <= (1ll << 24) && k <= (1ll << 24), "%s: dimension too large", op);
+    FSO_REQUIRE(m <= 65535 * 64 && rows <= (1ll << 24) && k <= (1ll << 24), "%s: dimension too large", op);
     FSO_REQUIRE((dtype == 0 || dtype == 1) && scale_dtype >= 0 && scale_dtype <= 2,
         "%s: dtype must be 0 (bf16) or 1 (fp16), scale_dtype 0, 1 or 2 (fp32)", op);
     if (m == 0) return 0;
@@ -769,6 +769,19 @@ static int check_int4(const char* op, int64_t m, int64_t rows, int64_t k, int64_
     FSO_REQUIRE(aligned16(x) && aligned16(codes) && aligned16(scale) && aligned16(zero),
         "%s: x, codes, scale and zero must be 16-byte aligned", op);
     return 0;
+}
+
+int fso_int4_pack_codes(const void* codes, void* packed, int64_t n, int64_t k, void* stream)
+{
+    FSO_REQUIRE(n > 0 && k > 0 && n <= (1ll << 24) && k <= (1ll << 24), "fso_int4_pack_codes: N and K must be in [1, 2^24]");
+    FSO_REQUIRE(k % 32 == 0, "fso_int4_pack_codes: K = %lld must be a multiple of 32", static_cast<long long>(k));
+    FSO_REQUIRE(codes && packed, "fso_int4_pack_codes: NULL pointer");
+    FSO_REQUIRE(aligned16(codes) && aligned16(packed), "fso_int4_pack_codes: codes and packed must be 16-byte aligned");
+    int64_t const vectors = n * (k / 32);
+    FSO_REQUIRE(vectors <= (1ll << 38), "fso_int4_pack_codes: N * K is too large for one launch");
+    int4_pack_kernel<<<blocks_for(vectors, 256), 256, 0, as_stream(stream)>>>(static_cast<uint4 const*>(codes),
+        static_cast<uint4*>(packed), vectors);
+    return launch_status("int4_pack_kernel");
 }
 
 int fso_int4_quantize(const void* w, void* codes, void* scale, void* zero, int64_t n, int64_t k, int64_t group, int64_t dtype,
@@ -797,15 +810,13 @@ int fso_int4_linear(const void* x, int64_t ldx, const void* codes, const void* s
     int const rc = check_int4("fso_int4_linear", m, n, k, group, dtype, scale_dtype, x, ldx, codes, scale, zero, y);
     if (rc != 0 || m == 0) return rc;
     Int4Params p{};
-    p.x = x;
-    p.ldx = ldx;
     p.scale_type = static_cast<int>(scale_dtype);
     p.bias = bias;
     p.out = y;
     p.m = static_cast<int>(m);
     p.k = static_cast<int>(k);
     p.out_cols = static_cast<int>(n);
-    return launch_int4(p, n, static_cast<uint8_t const*>(codes), scale, zero, group, dtype == 0, as_stream(stream));
+    return launch_int4(p, x, ldx, n, codes, scale, zero, group, dtype == 0, as_stream(stream));
 }
 
 int fso_int4_gated_linear(const void* x, int64_t ldx, const void* codes, const void* scale, const void* zero, void* h,
@@ -817,8 +828,6 @@ int fso_int4_gated_linear(const void* x, int64_t ldx, const void* codes, const v
     int const rc = check_int4("fso_int4_gated_linear", m, 2 * inter, k, group, dtype, scale_dtype, x, ldx, codes, scale, zero, h);
     if (rc != 0 || m == 0) return rc;
     Int4Params p{};
-    p.x = x;
-    p.ldx = ldx;
     p.scale_type = static_cast<int>(scale_dtype);
     p.out = h;
     p.m = static_cast<int>(m);
@@ -826,7 +835,7 @@ int fso_int4_gated_linear(const void* x, int64_t ldx, const void* codes, const v
     p.out_cols = static_cast<int>(inter);
     p.gated = 1;
     p.act = static_cast<int>(activation);
-    return launch_int4(p, 2 * inter, static_cast<uint8_t const*>(codes), scale, zero, group, dtype == 0, as_stream(stream));
+    return launch_int4(p, x, ldx, 2 * inter, codes, scale, zero, group, dtype == 0, as_stream(stream));
 }
 
 }  // extern "C"

@@ -26,7 +26,7 @@ ACTIVATIONS = tuple(_ops.GATE_ACTIVATIONS)
 GROUP_SIZES = (32, 64, 128, 256)       # of quantize_weight; prepare_weight takes any larger power of two as well
 _SCALE_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _MAX_DIM = 1 << 24
-_MAX_ROWS = 65535 * 8
+_MAX_ROWS = 65535 * 64
 
 
 def _by_halves(t: torch.Tensor) -> torch.Tensor:
@@ -47,17 +47,26 @@ def _rows_of(t: torch.Tensor, n: int) -> torch.Tensor:
 @dataclasses.dataclass(frozen=True, eq=False, repr=False)
 class Int4Weight:
     """One 4-bit weight: ``codes`` uint8 ``[N, K/2]``, ``scale`` bf16, fp16 or fp32 ``[N, K/group_size]``, ``zero`` uint8
-    of the same shape or None (8 everywhere). The kernels read them transposed and by halves of the rows, as ``scale_t``
-    and ``zero_t`` ``[K/group_size, 2 * half]``: ``half`` is half of N rounded up to a multiple of 16, the first half of the
-    rows starts at column 0 and the second at column ``half``."""
+    of the same shape or None (8 everywhere), as a checkpoint stores them. What the kernels read is ``packed``, the codes with
+    the even k of every eight in the lower four nibbles of a 32-bit word and the odd k in the upper four, and ``scale_t``
+    and ``zero_t`` ``[K/group_size, 2 * half]``, transposed and by halves of the rows: ``half`` is half of N rounded up to a
+    multiple of 16, the first half of the rows starts at column 0 and the second at column ``half``. ``codes``, ``scale`` and
+    ``zero`` are made of them when asked for."""
 
     arch: int
     in_features: int
     out_features: int
     group_size: int
-    codes: torch.Tensor
+    packed: torch.Tensor
     scale_t: torch.Tensor
     zero_t: Optional[torch.Tensor]
+
+    @property
+    def codes(self) -> torch.Tensor:
+        b = self.packed.view(self.out_features, -1, 4)      # bytes: k 0 2, 4 6, 1 3, 5 7
+        even = torch.stack((b[..., 0] & 15, b[..., 0] >> 4, b[..., 1] & 15, b[..., 1] >> 4), -1)
+        odd = torch.stack((b[..., 2] & 15, b[..., 2] >> 4, b[..., 3] & 15, b[..., 3] >> 4), -1)
+        return (even | (odd << 4)).flatten(1)
 
     @property
     def scale(self) -> torch.Tensor:
@@ -135,7 +144,7 @@ def _need_arch(op: str) -> None:
 def _complete(handle: Int4Weight) -> Int4Weight:
     """One empty plain launch behind whatever wrote the handle's tensors: a call on it starts to load the weight before
     its predecessor on the stream has finished, which is only safe when that predecessor did not write it."""
-    _ops.stream_fence(handle.codes.device)
+    _ops.stream_fence(handle.packed.device)
     return handle
 
 
@@ -196,8 +205,7 @@ def _int4_gated_linear_fake(x, codes, scale, zero, activation):
 def prepare_weight(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None) -> Int4Weight:
     """The handle of a weight that a checkpoint stores in 4 bits: ``codes`` uint8 ``[N, K/2]``, ``scale`` bf16, fp16 or
     fp32 ``[N, K/group]``, ``zero`` uint8 ``[N, K/group]`` with values 0..15 (None: 8 everywhere). The group size is a power
-    of two of at least 32. The codes are kept as they are (copied if they are not contiguous or off a 16-byte boundary),
-    scales and zero points are transposed. The values of ``zero`` are not looked at (that would synchronize)."""
+    of two of at least 32. All three are laid out anew for the kernels (one pass over each). The values of ``zero`` are not looked at (that would synchronize)."""
     ctx = "fso.int4.prepare_weight"
     for name, t in (("codes", codes), ("scale", scale), ("zero", zero)):
         if not isinstance(t, torch.Tensor) and not (name == "zero" and t is None):
@@ -211,7 +219,8 @@ def prepare_weight(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torc
     _check_weight(ctx, codes, scale_t, zero_t)
     _need_arch(ctx)
     k = 2 * int(codes.shape[1])
-    return _complete(Int4Weight(device_arch(), k, int(codes.shape[0]), k // int(scale_t.shape[0]), codes, scale_t, zero_t))
+    return _complete(Int4Weight(device_arch(), k, int(codes.shape[0]), k // int(scale_t.shape[0]), _ops.int4_pack_codes(codes),
+                                scale_t, zero_t))
 
 
 def quantize_weight(w: torch.Tensor, *, group_size: int = 128, zero_point: bool = False,
@@ -255,12 +264,12 @@ def linear(x: torch.Tensor, weight: Int4Weight, *, bias: Optional[torch.Tensor] 
     of the same shape."""
     x2 = _flatten(x, weight, "fso.int4.linear")
     if torch.compiler.is_compiling():
-        y = torch.ops.fish_scales_ops.int4_linear(x2, weight.codes, weight.scale_t, weight.zero_t, bias)
+        y = torch.ops.fish_scales_ops.int4_linear(x2, weight.packed, weight.scale_t, weight.zero_t, bias)
     else:
-        _check_x("fso.int4.linear", x2, weight.codes)
+        _check_x("fso.int4.linear", x2, weight.packed)
         if bias is not None:
             _check_bias("fso.int4.linear", bias, x2, weight.out_features)
-        y = _ops.int4_linear(x2, weight.codes, weight.scale_t, weight.zero_t, bias)
+        y = _ops.int4_linear(x2, weight.packed, weight.scale_t, weight.zero_t, bias)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.out_features)
 
 
@@ -270,9 +279,9 @@ def gated_linear(x: torch.Tensor, gate_up: Int4Weight, *, activation: str = "sil
     ``"silu"``, ``"gelu"`` (erf) or ``"gelu_tanh"``. Otherwise as :func:`linear`."""
     x2 = _flatten(x, gate_up, "fso.int4.gated_linear")
     if torch.compiler.is_compiling():
-        h = torch.ops.fish_scales_ops.int4_gated_linear(x2, gate_up.codes, gate_up.scale_t, gate_up.zero_t, activation)
+        h = torch.ops.fish_scales_ops.int4_gated_linear(x2, gate_up.packed, gate_up.scale_t, gate_up.zero_t, activation)
     else:
-        _check_gate("fso.int4.gated_linear", gate_up.codes, activation)
-        _check_x("fso.int4.gated_linear", x2, gate_up.codes)
-        h = _ops.int4_gated_linear(x2, gate_up.codes, gate_up.scale_t, gate_up.zero_t, _ops.GATE_ACTIVATIONS[activation])
+        _check_gate("fso.int4.gated_linear", gate_up.packed, activation)
+        _check_x("fso.int4.gated_linear", x2, gate_up.packed)
+        h = _ops.int4_gated_linear(x2, gate_up.packed, gate_up.scale_t, gate_up.zero_t, _ops.GATE_ACTIVATIONS[activation])
     return h if x.dim() == 2 else h.reshape(*x.shape[:-1], gate_up.out_features // 2)
