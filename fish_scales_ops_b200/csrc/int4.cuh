@@ -28,7 +28,7 @@ struct Int4Params {
     int out_cols;          // rows of the weight, or half of them when gated
     int gated;
     int act;
-    int steps;             // 128-wide steps of the contraction
+    int steps;             // 256-wide steps of the contraction
     int whole;             // CTAs at the front of the grid that take the whole contraction of a tile
     int splits;            // CTAs of a cluster, which share a tile of the others
     int steps_per_slice;
@@ -117,19 +117,19 @@ template <int N>
 struct Int4Cfg {
     static constexpr int kWorkers = 8;                   // warps that unpack and drain
     static constexpr int kThreads = 64 + 32 * kWorkers;  // TMA, MMA, workers
-    static constexpr int kCodeBytes = 128 * 64;          // 128 rows x 128 codes
-    static constexpr int kXBytes = N * 256;              // two tiles of N rows x 64 elements
-    static constexpr int kScaleOff = kCodeBytes + kXBytes;       // [half][group][64 rows], at most four groups
-    static constexpr int kZeroOff = kScaleOff + 2 * 4 * 64 * 4;
-    static constexpr int kStageBytes = (kZeroOff + 2 * 4 * 64 + 1023) / 1024 * 1024;
-    static constexpr int kStages = (108 * 1024) / kStageBytes < 8 ? (108 * 1024) / kStageBytes : 8;
+    static constexpr int kStep = 256;                    // of the contraction in a stage
+    static constexpr int kCodeBytes = 128 * kStep / 2;
+    static constexpr int kXBytes = N * kStep * 2;        // four tiles of N rows x 64 elements
+    static constexpr int kScaleOff = kCodeBytes + kXBytes;       // [half][group][64 rows], at most eight groups
+    static constexpr int kZeroOff = kScaleOff + 2 * 8 * 64 * 4;
+    static constexpr int kStageBytes = (kZeroOff + 2 * 8 * 64 + 1023) / 1024 * 1024;
+    static constexpr int kStages = (109 * 1024) / kStageBytes;
     static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 512;
-    // tensor memory: two buffers of unpacked weights (128 elements, 64 columns), then the accumulators of single groups
-    static constexpr int kD0 = 128;
-    static constexpr int kDBufs = N == 16 ? 8 : N == 32 ? 4 : 2;
-    static constexpr int kTmemCols = 256;
+    // tensor memory: the unpacked weights of a step (256 elements, 128 columns), then two buffers of group accumulators
+    static constexpr int kDCols = 64;
+    static constexpr int kTmemCols = 256;                // two CTAs share an SM's 512
     static constexpr int kRedStride = 132;               // floats between the rows of x in the sums
-    static_assert(kD0 + kDBufs * N <= kTmemCols, "two CTAs share an SM's tensor memory");
+    static_assert(kStages >= 2, "pipeline depth");
     static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
     static_assert(N * kRedStride * 4 <= kStages * kStageBytes, "the sums fit the stages");
 };
@@ -145,8 +145,12 @@ struct Int4Cfg {
 // of a cluster split the contraction of a tile where tiles are few or do not come out even, and each adds up a part of
 // the outputs over distributed shared memory, in a fixed order.
 //
-// GC: units of a step, i.e. groups inside its 128 elements (1 for groups of 128 and more).
-template <bool kBf16, int N, int GC>
+// What a step costs beside the unpacking (three waits, three arrivals, addresses: about a hundred instructions of a warp)
+// is paid once for 256 of the contraction; one buffer of unpacked weights is enough, since the MMAs of a step take less than
+// the unpacking of the next.
+//
+// U: units of a step that have sums of their own: its groups, or two halves of 128 where a group is longer.
+template <bool kBf16, int N, int U>
 __global__ void __launch_bounds__(Int4Cfg<N>::kThreads, 2)
 int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ CUtensorMap tm_hi,
     const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_scale, const __grid_constant__ CUtensorMap tm_zero,
@@ -161,11 +165,16 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
     uint32_t const bars = base + S * C::kStageBytes;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
-    auto afull_bar = [&](int a) { return bars + 8u * (2 * S + a); };
-    auto aempty_bar = [&](int a) { return bars + 8u * (2 * S + 2 + a); };
-    auto dfull_bar = [&](int d) { return bars + 8u * (2 * S + 4 + d); };
-    auto dempty_bar = [&](int d) { return bars + 8u * (2 * S + 4 + C::kDBufs + d); };
-    uint32_t const misc = S * C::kStageBytes + 8 * (2 * S + 4 + 2 * C::kDBufs);
+    uint32_t const afull_bar = bars + 16u * S, aempty_bar = afull_bar + 8;
+    auto dfull_bar = [&](int d) { return bars + 16u * S + 16 + 8u * d; };
+    auto dempty_bar = [&](int d) { return bars + 16u * S + 32 + 8u * d; };
+    uint32_t const misc = S * C::kStageBytes + 16 * S + 48;
+    // accumulators of so many units share a buffer, a wait and an arrival
+    constexpr int UB = U < C::kDCols / N ? U : C::kDCols / N;
+    static_assert(UB >= 1 && U % UB == 0, "batches of units");
+    // The MMAs of a step fill both buffers and go on when the workers have drained one. Where that is not all of the step, the
+    // workers drain it before they wait for its weights to be done with; otherwise after they have stored the next ones.
+    constexpr bool kDrainFirst = U / UB > 2;
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + misc);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(gbase + misc + 4);
 
@@ -186,11 +195,9 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), C::kWorkers + 1);
         }
-        for (int a = 0; a < 2; ++a) {
-            mbar_init(afull_bar(a), C::kWorkers);
-            mbar_init(aempty_bar(a), 1);
-        }
-        for (int d = 0; d < C::kDBufs; ++d) {
+        mbar_init(afull_bar, C::kWorkers);
+        mbar_init(aempty_bar, 1);
+        for (int d = 0; d < 2; ++d) {
             mbar_init(dfull_bar(d), 1);
             mbar_init(dempty_bar(d), C::kWorkers);
         }
@@ -212,25 +219,25 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
         // are fetched under the preceding kernel) and x
         if (elect_one()) {
             int const row0 = tile * 64;
-            int const box_groups = max(1, 128 >> p.group_shift);
+            int const box_groups = max(1, C::kStep >> p.group_shift);
             uint32_t const scale_bytes = box_groups * 64 * (p.scale_type == 2 ? 4 : 2), zero_bytes = box_groups * 64;
             uint32_t const bytes = C::kCodeBytes + C::kXBytes + 2 * scale_bytes + (p.has_zero ? 2 * zero_bytes : 0);
             auto load_weight = [&](int stage, int st) {
                 uint32_t const fb = full_bar(stage), dst = base + stage * C::kStageBytes;
-                int const g0 = (st * 128) >> p.group_shift;
+                int const g0 = (st * C::kStep) >> p.group_shift;
                 mbar_expect_tx(fb, bytes);
-                tma_load_2d(dst, &tm_lo, fb, st * 64, row0);
-                tma_load_2d(dst + 4096, &tm_hi, fb, st * 64, row0);
+                tma_load_2d(dst, &tm_lo, fb, st * (C::kStep / 2), row0);
+                tma_load_2d(dst + 8192, &tm_hi, fb, st * (C::kStep / 2), row0);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    tma_load_2d(dst + C::kScaleOff + h * 1024, &tm_scale, fb, row0 + h * p.half_cols, g0);
-                    if (p.has_zero) tma_load_2d(dst + C::kZeroOff + h * 256, &tm_zero, fb, row0 + h * p.half_cols, g0);
+                    tma_load_2d(dst + C::kScaleOff + h * 2048, &tm_scale, fb, row0 + h * p.half_cols, g0);
+                    if (p.has_zero) tma_load_2d(dst + C::kZeroOff + h * 512, &tm_zero, fb, row0 + h * p.half_cols, g0);
                 }
             };
             auto load_x = [&](int stage, int st) {
                 uint32_t const dst = base + stage * C::kStageBytes + C::kCodeBytes;
-                tma_load_2d(dst, &tm_x, full_bar(stage), st * 128, t0);
-                tma_load_2d(dst + N * 128, &tm_x, full_bar(stage), st * 128 + 64, t0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tma_load_2d(dst + i * (N * 128), &tm_x, full_bar(stage), st * C::kStep + i * 64, t0);
             };
             int const npre = min(S, step1 - step0);      // the first stages are free
             for (int i = 0; i < npre; ++i) load_weight(i, step0 + i);
@@ -256,17 +263,17 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
         // -------------------------------------------------------------------------------- MMA
         if (elect_one()) {
             constexpr uint32_t idesc = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (static_cast<uint32_t>(N >> 3) << 17) | ((128u >> 4) << 24);
-            int stage = 0, abuf = 0, dbuf = 0;
+            int stage = 0, dbuf = 0;
             uint32_t phase = 0, aphase = 0, dphase = 0;
             bool ok = true;
             for (int st = step0; ok && st < step1; ++st) {
-                if (!wait_or_abort(full_bar(stage), phase, abort_flag) || !wait_or_abort(afull_bar(abuf), aphase, abort_flag)) {
+                if (!wait_or_abort(full_bar(stage), phase, abort_flag) || !wait_or_abort(afull_bar, aphase, abort_flag)) {
                     record_abort(FSO_DEV_WAIT_MMA_FULL, abort_flag);
                     break;
                 }
                 uint64_t const bdesc = make_desc_sw128(base + stage * C::kStageBytes + C::kCodeBytes);
 #pragma unroll
-                for (int j = 0; j < GC; ++j) {
+                for (int j = 0; j < U / UB; ++j) {
                     if (!wait_or_abort(dempty_bar(dbuf), dphase ^ 1u, abort_flag)) {
                         record_abort(FSO_DEV_WAIT_MMA_TMEM, abort_flag);
                         ok = false;
@@ -274,24 +281,20 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
                     }
                     tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < 8 / GC; ++i) {
-                        int const kk = j * (8 / GC) + i;      // 16 elements of the contraction
-                        tc_mma_f16_ta(tmem + C::kD0 + dbuf * N, tmem + abuf * 64 + kk * 8,
-                            bdesc + static_cast<uint64_t>((kk >> 2) * (N * 128 / 16) + 2 * (kk & 3)), idesc, i > 0 ? 1u : 0u);
+                    for (int i = 0; i < 16 * UB / U; ++i) {
+                        int const kk = j * (16 * UB / U) + i;      // 16 elements of the contraction
+                        int const unit = i / (16 / U);
+                        tc_mma_f16_ta(tmem + 128 + dbuf * C::kDCols + unit * N, tmem + kk * 8,
+                            bdesc + static_cast<uint64_t>((kk >> 2) * (N * 128 / 16) + 2 * (kk & 3)), idesc, i % (16 / U) > 0 ? 1u : 0u);
                     }
                     tc_commit(dfull_bar(dbuf));
-                    if (++dbuf == C::kDBufs) {
-                        dbuf = 0;
-                        dphase ^= 1u;
-                    }
+                    dbuf ^= 1;
+                    dphase ^= dbuf ^ 1;
                 }
                 if (!ok) break;
-                tc_commit(aempty_bar(abuf));
+                tc_commit(aempty_bar);
                 tc_commit(empty_bar(stage));
-                if (++abuf == 2) {
-                    abuf = 0;
-                    aphase ^= 1u;
-                }
+                aphase ^= 1u;
                 if (++stage == S) {
                     stage = 0;
                     phase ^= 1u;
@@ -305,37 +308,41 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
         int const quarter = warp & 3, hh = (warp - 2) >> 2;
         int const row = quarter * 32 + lane, in_half = row & 63, half = row >> 6;
         uint32_t const lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        uint32_t const code_row = half * 4096 + in_half * 64, code_xor = (in_half >> 1) & 3;      // 64-byte swizzle
+        uint32_t const code_row = half * 8192 + in_half * 128;
         uint32_t const scale_width = p.scale_type == 2 ? 4 : 2;
-        uint32_t const scale_row = C::kScaleOff + half * 1024 + in_half * scale_width, zero_row = C::kZeroOff + half * 256 + in_half;
+        uint32_t const scale_row = C::kScaleOff + half * 2048 + in_half * scale_width, zero_row = C::kZeroOff + half * 512 + in_half;
+        int const unit_mask = U == 2 && p.group_shift >= 8 ? 0 : U - 1;      // units that share a longer group
         constexpr int kCols = N / 2;
         float acc[kCols] = {};
-        float scale_next[GC], scale_now[GC];
-        int stage = 0, abuf = 0, dbuf = 0;
+        float scale_next[U], scale_now[U];
+        int stage = 0, dbuf = 0;
         uint32_t phase = 0, aphase = 0, dphase = 0;
 
-        auto drain = [&]() -> bool {      // the groups of the step before, scaled
+        auto drain = [&]() -> bool {      // the units of the step before, scaled
 #pragma unroll
-            for (int j = 0; j < GC; ++j) {
+            for (int j = 0; j < U; j += UB) {
                 if (!wait_or_abort(dfull_bar(dbuf), dphase, abort_flag)) {
                     if (lane == 0) record_abort(FSO_DEV_WAIT_EPILOGUE, abort_flag);
                     return false;
                 }
                 __syncwarp();
                 tc_fence_after();
-                uint32_t r[kCols];
+                uint32_t r[UB * kCols];
 #pragma unroll
-                for (int c = 0; c < kCols; c += 8) tmem_ld_32x8(tmem + lanes + C::kD0 + dbuf * N + hh * kCols + c, r + c);
+                for (int u = 0; u < UB; ++u)
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 8)
+                        tmem_ld_32x8(tmem + lanes + 128 + dbuf * C::kDCols + u * N + hh * kCols + c, r + u * kCols + c);
                 tmem_ld_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(dempty_bar(dbuf));
 #pragma unroll
-                for (int c = 0; c < kCols; ++c) acc[c] = fmaf(scale_now[j], __uint_as_float(r[c]), acc[c]);
-                if (++dbuf == C::kDBufs) {
-                    dbuf = 0;
-                    dphase ^= 1u;
-                }
+                for (int u = 0; u < UB; ++u)
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) acc[c] = fmaf(scale_now[j + u], __uint_as_float(r[u * kCols + c]), acc[c]);
+                dbuf ^= 1;
+                dphase ^= dbuf ^ 1;
             }
             return true;
         };
@@ -349,51 +356,65 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
             }
             __syncwarp();
             uint32_t const src = base + stage * C::kStageBytes;
-            uint4 const c0 = lds_v4(src + code_row + (((2 * hh) ^ code_xor) << 4)), c1 = lds_v4(src + code_row + (((2 * hh + 1) ^ code_xor) << 4));
-            uint32_t zero2[2];      // of the two 32-wide parts of this half of the step
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                int const j = GC == 4 ? 2 * hh + q : GC == 2 ? hh : 0;
-                uint32_t const z = lds_u8(src + zero_row + j * 64);
-                zero2[q] = ((kBf16 ? 0x4300u : 0x6400u) + (p.has_zero ? z : 8u)) * 0x10001u;
-            }
-#pragma unroll
-            for (int j = 0; j < GC; ++j) {
-                uint32_t const at = src + scale_row + j * 64 * scale_width;
+            for (int j = 0; j < U; ++j) {
+                uint32_t const at = src + scale_row + (j & unit_mask) * 64 * scale_width;
                 uint32_t const upper = lds_u16(at + scale_width - 2), lower = lds_u16(at);
                 scale_next[j] = p.scale_type == 1 ? __half2float(__ushort_as_half(static_cast<uint16_t>(upper)))
                                                   : __uint_as_float(upper << 16 | (p.scale_type == 2 ? lower : 0u));
             }
-            uint32_t a[32];
-            uint32_t const words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) int4_unpack<kBf16>(words[j], zero2[j >> 2], a + 4 * j);
-            if (!wait_or_abort(aempty_bar(abuf), aphase ^ 1u, abort_flag)) {
-                if (lane == 0) record_abort(FSO_DEV_WAIT_MMA_TMEM, abort_flag);
-                ok = false;
-                break;
+            for (int b = 0; b < 2; ++b) {      // 64 of the contraction
+                int const part = 2 * hh + b;
+                uint4 const c0 = lds_v4(src + code_row + (((2 * part) ^ (in_half & 7)) << 4));
+                uint4 const c1 = lds_v4(src + code_row + (((2 * part + 1) ^ (in_half & 7)) << 4));
+                constexpr int kZeros = U == 8 ? 2 : 1;      // groups of these 64
+                uint32_t zero2[kZeros];
+#pragma unroll
+                for (int q = 0; q < kZeros; ++q) {
+                    int const j = U == 8 ? 2 * part + q : U == 4 ? part : part >> 1;
+                    uint32_t const z = lds_u8(src + zero_row + (j & unit_mask) * 64);
+                    zero2[q] = ((kBf16 ? 0x4300u : 0x6400u) + (p.has_zero ? z : 8u)) * 0x10001u;
+                }
+                uint32_t a[32];
+                uint32_t const words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) int4_unpack<kBf16>(words[j], zero2[j * kZeros >> 3], a + 4 * j);
+                if (b == 0) {
+                    if constexpr (kDrainFirst) {
+                        if (st > step0 && !drain()) {
+                            ok = false;
+                            break;
+                        }
+                    }
+                    if (!wait_or_abort(aempty_bar, aphase ^ 1u, abort_flag)) {
+                        if (lane == 0) record_abort(FSO_DEV_WAIT_MMA_TMEM, abort_flag);
+                        ok = false;
+                        break;
+                    }
+                    __syncwarp();
+                    tc_fence_after();
+                }
+                tmem_st_32x32(tmem + lanes + part * 32, a);
             }
-            __syncwarp();
-            tc_fence_after();
-            tmem_st_32x32(tmem + lanes + abuf * 64 + hh * 32, a);
+            if (!ok) break;
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(afull_bar(abuf));
+                mbar_arrive(afull_bar);
                 mbar_arrive(empty_bar(stage));
             }
-            if (++abuf == 2) {
-                abuf = 0;
-                aphase ^= 1u;
-            }
+            aphase ^= 1u;
             if (++stage == S) {
                 stage = 0;
                 phase ^= 1u;
             }
-            if (st > step0) ok = drain();
+            if constexpr (!kDrainFirst) {
+                if (st > step0) ok = drain();
+            }
 #pragma unroll
-            for (int j = 0; j < GC; ++j) scale_now[j] = scale_next[j];
+            for (int j = 0; j < U; ++j) scale_now[j] = scale_next[j];
         }
         if (ok && step1 > step0) ok = drain();
         // every MMA and every copy is done: the sums of this slice go where the stages were
@@ -517,27 +538,10 @@ __global__ void int4_quantize_kernel(const uint4* __restrict__ w, uint32_t* __re
     }
 }
 
-// Tensor map of the codes [rows, k / 2] in boxes of 64 bytes x 64 rows with the 64-byte swizzle.
+// Tensor map of the codes [rows, k / 2] in boxes of 128 bytes x 64 rows with the 128-byte swizzle.
 inline int make_codes_map(CUtensorMap* map, const uint8_t* codes, int64_t rows, int64_t k)
 {
-    EncodeTiledFn fn = encode_tiled_fn();
-    if (fn == nullptr) {
-        set_error("cuTensorMapEncodeTiled is not available from this driver");
-        return FSO_ERR_UNSUPPORTED;
-    }
-    cuuint64_t const dims[2] = {static_cast<cuuint64_t>(k / 2), static_cast<cuuint64_t>(rows)};
-    cuuint64_t const strides[1] = {static_cast<cuuint64_t>(k / 2)};
-    cuuint32_t const box[2] = {64u, 64u};
-    cuuint32_t const estr[2] = {1u, 1u};
-    CUresult const r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, estr,
-        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) {
-        set_error("cuTensorMapEncodeTiled failed with CUresult %d (codes, %lld x %lld)", static_cast<int>(r),
-            static_cast<long long>(rows), static_cast<long long>(k));
-        return FSO_ERR_INTERNAL;
-    }
-    return 0;
+    return make_operand_map(map, codes, rows, k / 2, 64);
 }
 
 // Tensor map of scale or zero [groups, 2 * half_cols] in boxes of 64 rows of the weight x box_groups.
@@ -588,12 +592,12 @@ inline unsigned int4_schedule(int tiles, int sms, Int4Params& p)
     return static_cast<unsigned>(p.whole + (tiles - p.whole) * p.splits);
 }
 
-template <bool kBf16, int N, int GC>
+template <bool kBf16, int N, int U>
 inline int launch_int4_inst(CUtensorMap const (&maps)[5], Int4Params const& p, dim3 grid, cudaStream_t stream)
 {
     using C = Int4Cfg<N>;
     static std::atomic<uint64_t> done{0};
-    auto kernel = int4_kernel<kBf16, N, GC>;
+    auto kernel = int4_kernel<kBf16, N, U>;
     int const rc = ensure_smem_attr(kernel, C::kSmemBytes, done);
     if (rc != 0) return rc;
     cudaLaunchConfig_t cfg{};
@@ -615,9 +619,9 @@ inline int launch_int4_inst(CUtensorMap const (&maps)[5], Int4Params const& p, d
 template <bool kBf16, int N>
 inline int launch_int4_group(int64_t group, CUtensorMap const (&maps)[5], Int4Params const& p, dim3 grid, cudaStream_t stream)
 {
-    return group == 32 ? launch_int4_inst<kBf16, N, 4>(maps, p, grid, stream)
-        : group == 64 ? launch_int4_inst<kBf16, N, 2>(maps, p, grid, stream)
-                      : launch_int4_inst<kBf16, N, 1>(maps, p, grid, stream);
+    return group == 32 ? launch_int4_inst<kBf16, N, 8>(maps, p, grid, stream)
+        : group == 64 ? launch_int4_inst<kBf16, N, 4>(maps, p, grid, stream)
+                      : launch_int4_inst<kBf16, N, 2>(maps, p, grid, stream);
 }
 
 template <bool kBf16>
@@ -639,11 +643,11 @@ inline int launch_int4(Int4Params p, const void* x, int64_t ldx, int64_t rows, c
     p.rows0 = static_cast<int>((rows + 1) / 2);
     p.rows1 = static_cast<int>(rows - p.rows0);
     p.half_cols = static_cast<int>(int4_half_cols(rows));
-    p.steps = (p.k + 127) / 128;
+    p.steps = (p.k + 255) / 256;
     int const chunks = (p.m + 63) / 64;
     p.chunk_rows = (p.m + chunks - 1) / chunks;
     int const n = (p.chunk_rows + 15) / 16 * 16;
-    int const box_groups = static_cast<int>(std::max<int64_t>(1, 128 / group));
+    int const box_groups = static_cast<int>(std::max<int64_t>(1, 256 / group));
     int64_t const groups = p.k >> p.group_shift;
     uint8_t const* const c = static_cast<uint8_t const*>(codes);
     CUtensorMap maps[5];
