@@ -793,18 +793,27 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_constan
             if (col >= p.inter) continue;
             int const at = row * C::kRedStride + in_tile;
             float g[4] = {}, u[4] = {};
-            for (int r = 0; r < p.splits; ++r) {
-                float4 a, b;
-                if (p.splits == 1) {
-                    a = *reinterpret_cast<float4 const*>(red + at);
-                    b = *reinterpret_cast<float4 const*>(red + at + 64);
-                } else {
-                    uint32_t const peer = map_to_cta(red_addr + 4u * at, r);
-                    a = ld_cluster_f32x4(peer);
-                    b = ld_cluster_f32x4(peer + 256u);
+            if (p.splits == 1) {
+                float4 const a = *reinterpret_cast<float4 const*>(red + at), b = *reinterpret_cast<float4 const*>(red + at + 64);
+                g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
+                u[0] = b.x; u[1] = b.y; u[2] = b.z; u[3] = b.w;
+            } else {      // all loads first: one trip to the other CTAs' memory instead of one for each
+                float4 a[8], b[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    if (r < p.splits) {
+                        uint32_t const peer = map_to_cta(red_addr + 4u * at, r);
+                        a[r] = ld_cluster_f32x4(peer);
+                        b[r] = ld_cluster_f32x4(peer + 256u);
+                    }
                 }
-                g[0] += a.x; g[1] += a.y; g[2] += a.z; g[3] += a.w;
-                u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    if (r < p.splits) {
+                        g[0] += a[r].x; g[1] += a[r].y; g[2] += a[r].z; g[3] += a[r].w;
+                        u[0] += b[r].x; u[1] += b[r].y; u[2] += b[r].z; u[3] += b[r].w;
+                    }
+                }
             }
             int64_t const out_row = row0 + row;
             finish_four<kBf16>(g, u, p.act, p.save_hi, p.save_lo, out_row * 2 * p.half_cols + col, p.half_cols, p.out,

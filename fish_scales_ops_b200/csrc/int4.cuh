@@ -438,8 +438,13 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
         uint32_t const red_addr = smem_u32(red);
         auto sum_of = [&](int r, int c) {
             if (splits == 1) return red[r * C::kRedStride + c];
-            float v = 0.f;
-            for (int i = 0; i < splits; ++i) v += ld_cluster_f32(map_to_cta(red_addr + 4u * (r * C::kRedStride + c), i));
+            float part[8], v = 0.f;      // all loads first: one trip to the other CTAs' memory instead of one for each
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < splits) part[i] = ld_cluster_f32(map_to_cta(red_addr + 4u * (r * C::kRedStride + c), i));
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < splits) v += part[i];
             return v;
         };
         int const cols = p.gated ? 64 : 128;
