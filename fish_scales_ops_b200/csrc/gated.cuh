@@ -601,10 +601,10 @@ gated16_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
 // ------------------------------------------------------------------------------------------------ few rows
 //
 // The forward pass where 256 x 256 tiles are too coarse: 64 rows of G and the same 64 rows of U on MMA-M, up to 256 rows of x
-// (a multiple of 16) on MMA-N, one tile for each CTA. Up to 128 rows the weight bytes are the cost, and two CTAs share
-// an SM, so that more than a hundred kilobytes of its weights are on their way at any time. Where the tiles leave SMs
-// without work the CTAs of a cluster split the contraction, and each adds up its part of the outputs over distributed
-// shared memory, in a fixed order.
+// (a multiple of 16) on MMA-N, one tile for each CTA. Up to 128 rows the weight bytes are the cost, and a deep ring keeps
+// more than a hundred kilobytes of an SM's weights on their way: one CTA with all of its shared memory where there is
+// one for each SM, two that share it where there are more. Where the tiles leave SMs without work the CTAs of a cluster
+// split the contraction, and each adds up its part of the outputs over distributed shared memory, in a fixed order.
 // Nothing is read before the preceding kernel has finished: unlike a prepared weight, gate_up may be its output.
 template <int BN>
 struct GatedRowsCfg {
@@ -612,19 +612,23 @@ struct GatedRowsCfg {
     static constexpr int kABytes = 128 * 128;
     static constexpr int kBBytes = BN * 128;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kBlocks = BN <= 128 ? 2 : 1;      // CTAs that share an SM
-    static constexpr int kStages = (220 * 1024 / kBlocks) / kStageBytes;
-    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+    static constexpr int kBlocks = BN <= 128 ? 2 : 1;      // CTAs that can share an SM
+    // stages of a CTA that has its SM to itself, and of one that shares it
+    static constexpr int kStagesAlone = (220 * 1024) / kStageBytes;
+    static constexpr int kStagesShared = (110 * 1024) / kStageBytes;
+    static constexpr int smem_bytes(int stages) { return stages * kStageBytes + 1024 + 512; }
     static constexpr int kRedStride = 132;     // floats between the rows of x in the sums of a slice
     static constexpr int kTmemCols = BN < 32 ? 32 : BN;
-    static_assert(kBlocks * (kSmemBytes + 1024) <= 228 * 1024, "CTAs of an SM");
-    static_assert(BN * kRedStride * 4 <= kStages * kStageBytes, "the sums fit the stages");
+    static_assert(smem_bytes(kStagesAlone) + 1024 <= 228 * 1024 && 2 * (smem_bytes(kStagesShared) + 1024) <= 228 * 1024, "shared memory");
+    static_assert(16 * kStagesAlone + 16 <= 512, "barriers");
+    static_assert(BN * kRedStride * 4 <= (kBlocks == 2 ? kStagesShared : kStagesAlone) * kStageBytes, "the sums fit the stages");
 };
 
 struct GatedRowsParams {
     int t, inter, act;
     int n;               // rows of x in a tile, a multiple of 16 and at most BN
     int kb_total, kb_per_split, splits;
+    int stages;
     int vec;             // rows of `out` start on 8-byte boundaries
     void* out;
     uint16_t* save_hi;
@@ -665,7 +669,7 @@ gated_rows_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_constan
     const __grid_constant__ CUtensorMap tm_x, const GatedRowsParams p)
 {
     using C = GatedRowsCfg<BN>;
-    constexpr int S = C::kStages;
+    int const S = p.stages;
     extern __shared__ uint8_t smem_raw[];
     uint32_t const raw = smem_u32(smem_raw);
     uint32_t const base = (raw + 1023u) & ~1023u;
@@ -988,13 +992,15 @@ inline Gated16Plan plan_gated16_forward(int64_t t, int64_t k, int64_t inter, int
     int const row_tiles = tiles_of(t, 256), weight_tiles = tiles_of(inter, 64);
     int const n = static_cast<int>((tiles_of(t, row_tiles) + 15) / 16 * 16);
     int64_t const tiles = static_cast<int64_t>(row_tiles) * weight_tiles;
-    int const slots = n <= 128 ? 2 * sms : sms;
-    // slices: as many as all SMs need to have work, at most eight (the portable cluster size), of at least four blocks, none
-    // empty
+    int const slots = n <= 128 && tiles > sms ? 2 * sms : sms;
+    // Slices of at least four blocks: as many as SMs can take, at most four, each CTA with an SM to itself and its whole shared
+    // memory as a ring; a handful of tiles in eight slices (the portable cluster size), whose CTAs share SMs, because
+    // not all GPCs find eight free SMs twice.
+    int const limit = n <= 128 && tiles * 8 <= sms ? 8 : 4;
     int s = 1;
-    while (s < 8 && tiles * s * 2 <= (n <= 128 ? 3 * sms : sms) && (s + 1) * 4 <= p.kb) ++s;
+    while (s < limit && tiles * (s + 1) <= sms && (s + 1) * 4 <= p.kb) ++s;
     int const per = tiles_of(p.kb, s);
-    double const rows_us = std::ceil(static_cast<double>(tiles * s) / slots) * (per * std::max(264, 2 * n) / 1550.0 * (n <= 128 ? 2 : 1)
+    double const rows_us = std::ceil(static_cast<double>(tiles * s) / slots) * (per * std::max(264, 2 * n) / 1550.0 * (slots > sms ? 2 : 1)
         + 2.0 + 0.035 * n) + 3.0;
     // pairs
     p.tiles_m = tiles_of(t, 256);
@@ -1011,7 +1017,7 @@ inline Gated16Plan plan_gated16_forward(int64_t t, int64_t k, int64_t inter, int
             pair_s = q;
         }
     }
-    bool const rows = t <= 128 || (forced_gated_kernel() == 0 ? rows_us < pair_us : forced_gated_kernel() == 2);
+    bool const rows = t <= 128 || (row_tiles <= 1024 && (forced_gated_kernel() == 0 ? rows_us < pair_us : forced_gated_kernel() == 2));
     p.rows_n = rows ? n : 0;
     p.kb_per_split = rows ? per : tiles_of(p.kb, pair_s);
     p.splits = tiles_of(p.kb, p.kb_per_split);
@@ -1104,7 +1110,7 @@ inline int launch_gated_rows(const void* x, int64_t ldx, const void* gate_up, in
     using C = GatedRowsCfg<BN>;
     static std::atomic<uint64_t> done{0};
     auto kernel = gated_rows_kernel<BN, kBf16>;
-    int rc = ensure_smem_attr(kernel, C::kSmemBytes, done);
+    int rc = ensure_smem_attr(kernel, C::smem_bytes(C::kStagesAlone), done);
     if (rc != 0) return rc;
     uint16_t const* const w = static_cast<uint16_t const*>(gate_up);
     CUtensorMap mg, mu, mx;
@@ -1113,10 +1119,12 @@ inline int launch_gated_rows(const void* x, int64_t ldx, const void* gate_up, in
     if (rc == 0) rc = make_map16(&mx, x, p.t, k, ldx, p.n);
     if (rc != 0) return rc;
     int const tiles = (p.inter + 63) / 64, row_tiles = (p.t + p.n - 1) / p.n;
+    bool const alone = C::kBlocks == 1 || (p.splits <= 4 && tiles * row_tiles * p.splits <= sm_count());
+    p.stages = alone ? C::kStagesAlone : C::kStagesShared;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.splits), static_cast<unsigned>(row_tiles), 1);
     cfg.blockDim = dim3(C::kThreads, 1, 1);
-    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.dynamicSmemBytes = static_cast<size_t>(C::smem_bytes(p.stages));
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
