@@ -371,12 +371,6 @@ def gated_saved_cols(inter: int) -> int:
     return 6 * _align(inter, 16)
 
 
-def _saved_parts(saved, t: int, inter: int):
-    """Addresses of the upper 16 and of the lower 8 bits in the one buffer of the saved projections."""
-    p = saved.data_ptr()
-    return p, p + 4 * t * _align(inter, 16)
-
-
 def gated_linear(x, gate_up, activation: int, save: bool):
     """x [T, K], gate_up [2I, K] -> (h [T, I], saved projections as uint8 [T, gated_saved_cols(I)], None without
     ``save``)."""
@@ -389,33 +383,39 @@ def gated_linear(x, gate_up, activation: int, save: bool):
         with on_device(x.device):
             need = _gated_ws_bytes("fso_gated_linear_ws_bytes", t, k, inter, x.get_device())
             ws = x.new_empty((need,), dtype=torch.uint8) if need else None
-            hi, lo = _saved_parts(saved, t, inter) if save else (None, None)
-            rc = call_on(x, lib().fso_gated_linear, x.data_ptr(), ldx, gate_up.data_ptr(), h.data_ptr(), hi, lo, t, k, inter,
-                         DTYPES_16[x.dtype], activation, None if ws is None else ws.data_ptr(), need)
+            # the saved buffer: the upper 16 bits of all rows, then the lower 8
+            hi = saved.data_ptr() if save else None
+            rc = call_on(x, lib().fso_gated_linear, x.data_ptr(), ldx, gate_up.data_ptr(), h.data_ptr(), hi,
+                         hi + 4 * t * _align(inter, 16) if save else None, t, k, inter, DTYPES_16[x.dtype], activation,
+                         None if ws is None else ws.data_ptr(), need)
         if rc != 0:
             check(rc, "fso_gated_linear")
     return h, saved
 
 
 def gated_linear_backward(dh, x, gate_up, saved, activation: int, need_x: bool, need_w: bool):
-    """(dx [T, K] or empty, dgate_up [2I, K] or empty) for dh [T, I]."""
+    """(dx [T, K] or None, dgate_up [2I, K] or None) for dh [T, I]. Autograd calls this in a thread of its own, whose caches are
+    cold: it does as little as it can."""
     t, k = x.shape
+    if t == 0:
+        return x.new_empty((0, k)) if need_x else None, gate_up.new_zeros(gate_up.shape) if need_w else None
     inter = gate_up.shape[0] // 2
-    dx = x.new_empty((t if need_x else 0, k))
-    dw = (x.new_empty if t > 0 else x.new_zeros)((2 * inter if need_w else 0, k))
-    if t > 0 and (need_x or need_w):
-        x, ldx = rows_in_place(x)
-        if (inter > 1 and dh.stride(1) != 1) or (t > 1 and dh.stride(0) < inter):
-            dh = dh.contiguous()
-        with on_device(x.device):
-            need = _gated_ws_bytes("fso_gated_linear_backward_ws_bytes", t, k, inter, x.get_device())
-            ws = x.new_empty((need,), dtype=torch.uint8)
-            hi, lo = _saved_parts(saved, t, inter)
-            rc = call_on(x, lib().fso_gated_linear_backward, dh.data_ptr(), dh.stride(0) if t > 1 else inter, x.data_ptr(), ldx,
-                         gate_up.data_ptr(), hi, lo, dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None, t, k,
-                         inter, DTYPES_16[x.dtype], activation, ws.data_ptr(), need)
-        if rc != 0:
-            check(rc, "fso_gated_linear_backward")
+    x, ldx = rows_in_place(x)
+    if not dh.is_contiguous() and ((inter > 1 and dh.stride(1) != 1) or (t > 1 and dh.stride(0) < inter)):
+        dh = dh.contiguous()
+    dev = x.get_device()
+    with on_device(dev):
+        need = _gated_ws_bytes("fso_gated_linear_backward_ws_bytes", t, k, inter, dev)
+        dx = x.new_empty((t, k)) if need_x else None
+        dw = torch.empty_like(gate_up) if need_w else None
+        ws = saved.new_empty(need)
+        hi = saved.data_ptr()
+        rc = lib().fso_gated_linear_backward(dh.data_ptr(), dh.stride(0) if t > 1 else inter, x.data_ptr(), ldx, gate_up.data_ptr(),
+                                             hi, hi + 4 * t * _align(inter, 16), dx.data_ptr() if need_x else None,
+                                             dw.data_ptr() if need_w else None, t, k, inter, DTYPES_16[x.dtype], activation,
+                                             ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        check(rc, "fso_gated_linear_backward")
     return dx, dw
 
 

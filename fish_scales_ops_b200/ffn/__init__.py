@@ -66,7 +66,9 @@ def _gated_linear_backward_body(dh, x, gate_up, saved, activation, need_x, need_
     if tuple(saved.shape) != (t, cols) or saved.dtype != torch.uint8 or saved.device != x.device or not saved.is_contiguous():
         _refuse(op, f"saved must be the uint8 [{t}, {cols}] that fish_scales_ops::gated_linear returned with save, got "
                     f"{saved.dtype} {tuple(saved.shape)}")
-    return _ops.gated_linear_backward(dh, x, gate_up, saved, _ops.GATE_ACTIVATIONS[activation], need_x, need_w)
+    dx, dw = _ops.gated_linear_backward(dh, x, gate_up, saved, _ops.GATE_ACTIVATIONS[activation], need_x, need_w)
+    empty = x.new_empty((0, x.shape[1]))
+    return dx if need_x else empty, dw if need_w else empty
 
 
 _gated_linear_op = torch.library.custom_op(
@@ -105,17 +107,13 @@ def _setup_context(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
-def _gradients(backward, ctx, dh):
-    x, gate_up, saved = ctx.saved_tensors
-    need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-    if dh is None or not (need_x or need_w):
-        return None, None
-    dx, dw = backward(dh, x, gate_up, saved, ctx.activation, need_x, need_w)
-    return dx if need_x else None, dw if need_w else None
-
-
 def _op_backward(ctx, dh, *_):
-    return (*_gradients(torch.ops.fish_scales_ops.gated_linear_backward, ctx, dh), None, None)
+    x, gate_up, saved = ctx.saved_tensors
+    need_x, need_w = ctx.needs_input_grad[:2]
+    if dh is None or not (need_x or need_w):
+        return None, None, None, None
+    dx, dw = torch.ops.fish_scales_ops.gated_linear_backward(dh, x, gate_up, saved, ctx.activation, need_x, need_w)
+    return dx if need_x else None, dw if need_w else None, None, None
 
 
 _gated_linear_op.register_autograd(_op_backward, setup_context=_setup_context)
@@ -128,25 +126,27 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_up, activation):
         _check("fso.ffn.gated_linear", x, gate_up, activation)
-        h, saved = _ops.gated_linear(x, gate_up, _ops.GATE_ACTIVATIONS[activation], True)
+        act = _ops.GATE_ACTIVATIONS[activation]
+        h, saved = _ops.gated_linear(x, gate_up, act, True)
         ctx.save_for_backward(x, gate_up, saved)
-        ctx.activation = activation
+        ctx.act = act
         return h
 
     @staticmethod
     def backward(ctx, dh):
         if torch.is_grad_enabled():      # create_graph: the gradients come with a node that refuses to be differentiated
             return _differentiable_once(ctx, dh)
-        return (*_gradients(_eager_backward, ctx, dh), None)
+        return _eager_backward(ctx, dh)
 
 
-@torch.autograd.function.once_differentiable
-def _differentiable_once(ctx, dh):
-    return (*_gradients(_eager_backward, ctx, dh), None)
+def _eager_backward(ctx, dh):
+    x, gate_up, saved = ctx.saved_tensors
+    need_x, need_w, _ = ctx.needs_input_grad
+    dx, dw = _ops.gated_linear_backward(dh, x, gate_up, saved, ctx.act, need_x, need_w)
+    return dx, dw, None
 
 
-def _eager_backward(dh, x, gate_up, saved, activation, need_x, need_w):
-    return _ops.gated_linear_backward(dh, x, gate_up, saved, _ops.GATE_ACTIVATIONS[activation], need_x, need_w)
+_differentiable_once = torch.autograd.function.once_differentiable(_eager_backward)
 
 
 # ------------------------------------------------------------------------------------------------ public functions
