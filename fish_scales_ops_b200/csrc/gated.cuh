@@ -102,7 +102,8 @@ __device__ __forceinline__ void gate_value_slope(float g, float& a, float& s)
         dp = g * 0.39894228040143267794f * __expf(-0.5f * g * g);
     } else {
         p = logistic(2.f * kGeluC * (g + kGeluCubic * g * g * g));
-        dp = g * p * (1.f - p) * 2.f * kGeluC * (1.f + 3.f * kGeluCubic * g * g);
+        float const c = fminf(fabsf(g), 30.f);      // p is 0 or 1 long before that, and the square of a large g is infinite
+        dp = g * p * (1.f - p) * 2.f * kGeluC * (1.f + 3.f * kGeluCubic * c * c);
     }
     a = g * p;
     s = p + dp;

@@ -10,6 +10,7 @@ pytestmark = pytest.mark.gpu
 
 SIZES = [(1, 8, 1), (1, 64, 128), (3, 72, 17), (16, 4096, 40), (17, 520, 300), (64, 128, 64), (65, 264, 65), (100, 2048, 33),
          (128, 256, 256), (129, 1032, 130), (257, 64, 129), (300, 200, 1000), (513, 136, 264), (1030, 72, 520)]
+SPLIT = [(512, 7168, 256), (500, 7168, 251), (260, 4104, 24)]      # few tiles, long contractions: sums of slices
 
 
 def _case(t, k, i, dtype, seed=0):
@@ -25,7 +26,7 @@ def _grads(fso, x, w, dh, act):
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES, ids=["bf16", "fp16"])
-@pytest.mark.parametrize("t,k,i", SIZES)
+@pytest.mark.parametrize("t,k,i", SIZES + SPLIT)
 def test_forward_and_gradients(fso, device_ok, t, k, i, dtype):
     act = R.ACTIVATIONS[(t + i) % 3]
     x, w, dh = _case(t, k, i, dtype)
@@ -126,6 +127,24 @@ def test_extreme_values_stay_in_their_row(fso, device_ok):
         big, bound, _, _ = R.gated(y[7:8], w, act)
         R.inside(fso.ffn.gated_linear(y[7:8], w, activation=act), big, bound, act)
         assert torch.isfinite(torch.cat(_grads(fso, y[7:8], w, dh[7:8], act)[:2], 1)).all()
+
+
+@pytest.mark.parametrize("act", R.ACTIVATIONS)
+def test_gates_of_any_finite_size(fso, device_ok, act):
+    """Gates up to 1e30, whose squares fp32 does not hold: there act(g) is g or 0 and its slope 1 or 0. dg and du are rounded
+    once and so is their sum, g and u are in 24 bits, and 1e-5 is for the activation's own arithmetic."""
+    x = torch.tensor([[s * 10.0 ** e] + [0.0] * 7 for e in (5, 13, 19, 20, 30) for s in (1, -1)], dtype=torch.bfloat16).cuda()
+    w = torch.zeros(2, 8, dtype=torch.bfloat16, device="cuda")
+    w[0, 0], w[1, 0] = 1.0, 2.0 ** -100      # g = x, u = 2^-100 x
+    dh = torch.full((10, 1), 2.0 ** -20, dtype=torch.bfloat16, device="cuda")
+    xr = x.detach().requires_grad_()
+    h = fso.ffn.gated_linear(xr, w, activation=act)
+    (dx,) = torch.autograd.grad(h, xr, dh)
+    g = x[:, 0].double().clamp(min=0)
+    want, slope = g * g * 2.0 ** -100, 2 * g * 2.0 ** -120
+    he = R.half_step(torch.bfloat16)
+    assert ((h[:, 0].double() - want).abs() <= (he + 1e-5) * want).all()
+    assert ((dx[:, 0].double() - slope).abs() <= (2 * he + he * he + 2.0 ** -14 + 1e-5) * slope).all()
 
 
 def test_same_bits_every_time_and_on_another_stream(fso, device_ok):
