@@ -490,7 +490,8 @@ __global__ void int4_pack_kernel(const uint4* __restrict__ in, uint4* __restrict
 //
 // A group is group / 8 neighbouring lanes of eight weights each. Steps are amax / 7 around code 8, or (hi - lo) / 15 with
 // zero inside [lo, hi] and the zero point next to -lo / step; the step is rounded to its stored type first, so that the
-// codes are the nearest ones for the scale that will multiply them. A group whose step rounds to zero gets code = zero.
+// codes are the nearest ones for the scale that will multiply them. A group whose step rounds to zero gets code = zero, one
+// with a NaN or an infinity a scale that is not a number, so that its row's products show it.
 __device__ __forceinline__ float stored_scale(float v, int type)
 {
     if (type == 0) return __bfloat162float(__float2bfloat16_rn(v));
@@ -513,17 +514,19 @@ __global__ void int4_quantize_kernel(const uint4* __restrict__ w, uint32_t* __re
         v[2 * j] = f.x;
         v[2 * j + 1] = f.y;
     }
-    float lo = 0.f, hi = 0.f;
+    float lo = 0.f, hi = 0.f, nan = 0.f;      // minima and maxima pass over a NaN: 0 * v keeps it
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         lo = fminf(lo, v[j]);
         hi = fmaxf(hi, v[j]);
+        nan += 0.f * v[j];
     }
     for (int o = lanes / 2; o > 0; o >>= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        nan += __shfl_xor_sync(0xffffffffu, nan, o);
     }
-    float const step = stored_scale(zero != nullptr ? (hi - lo) / 15.f : fmaxf(-lo, hi) / 7.f, scale_type);
+    float const step = stored_scale((zero != nullptr ? (hi - lo) / 15.f : fmaxf(-lo, hi) / 7.f) + nan, scale_type);
     int const z = zero == nullptr ? 8 : step > 0.f ? min(15, max(0, __float2int_rn(-lo / step))) : 0;
     uint32_t packed = 0;
 #pragma unroll

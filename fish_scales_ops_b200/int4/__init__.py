@@ -51,7 +51,11 @@ class Int4Weight:
     the even k of every eight in the lower four nibbles of a 32-bit word and the odd k in the upper four, and ``scale_t``
     and ``zero_t`` ``[K/group_size, 2 * half]``, transposed and by halves of the rows: ``half`` is half of N rounded up to a
     multiple of 16, the first half of the rows starts at column 0 and the second at column ``half``. ``codes``, ``scale`` and
-    ``zero`` are made of them when asked for."""
+    ``zero`` are made of them when asked for.
+
+    A call starts to load the weight before the kernel ahead of it on the stream has finished. Whoever rewrites a handle's
+    tensors in place has a kernel that does not write them run between that and the next call (the functions that make a
+    handle see to it themselves)."""
 
     arch: int
     in_features: int
@@ -205,7 +209,8 @@ def _int4_gated_linear_fake(x, codes, scale, zero, activation):
 def prepare_weight(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None) -> Int4Weight:
     """The handle of a weight that a checkpoint stores in 4 bits: ``codes`` uint8 ``[N, K/2]``, ``scale`` bf16, fp16 or
     fp32 ``[N, K/group]``, ``zero`` uint8 ``[N, K/group]`` with values 0..15 (None: 8 everywhere). The group size is a power
-    of two of at least 32. All three are laid out anew for the kernels (one pass over each). The values of ``zero`` are not looked at (that would synchronize)."""
+    of two of at least 32. All three are laid out anew for the kernels (one pass over each). The values of ``zero`` are not
+    looked at (that would synchronize)."""
     ctx = "fso.int4.prepare_weight"
     for name, t in (("codes", codes), ("scale", scale), ("zero", zero)):
         if not isinstance(t, torch.Tensor) and not (name == "zero" and t is None):
@@ -229,7 +234,7 @@ def quantize_weight(w: torch.Tensor, *, group_size: int = 128, zero_point: bool 
     ``zero_point`` the step is ``amax / 7`` and codes run from 1 to 15 around 8; with it the step is ``(hi - lo) / 15``
     for the group's range with zero inside, and the zero point ``round(-lo / step)``. The step is rounded to
     ``scale_dtype`` (default: the weight's type) before the codes are taken. ``group_size`` is one of 32, 64, 128, 256
-    and divides K."""
+    and divides K. A group that holds a NaN or an infinity gets a scale that is not a number."""
     ctx = "fso.int4.quantize_weight"
     if not isinstance(w, torch.Tensor) or w.dim() != 2 or w.dtype not in _ops.DTYPES_16 or not w.is_cuda:
         raise ValueError(f"{ctx}: w must be a CUDA bf16 or fp16 [N, K] tensor")

@@ -290,18 +290,21 @@ int fso_gated_linear_backward(const void* dh, int64_t ldh, const void* x, int64_
  *
  * W[n, k] = scale[n, k / group] * (code[n, k] - zero[n, k / group]); codes in 32-bit words of eight consecutive k (even k
  * in the lower four nibbles, odd k in the upper four, each in their order), rows of K / 2 bytes; fso_int4_pack_codes makes
- * them of a checkpoint's codes, two in a byte with the even k in the lower four bits. scale, bf16 (0), fp16 (1) or fp32 (2), lies transposed and by halves of the rows, so that the
+ * them of a checkpoint's codes, two in a byte with the even k in the lower four bits. scale, bf16 (0), fp16 (1) or
+ * fp32 (2), lies transposed and by halves of the rows, so that the
  * scales of neighbouring rows are read together from 16-byte boundaries: [K / group, 2 * half] with half = (N + 1) / 2 rounded
  * up to a multiple of 16; row n of the first (N + 1) / 2 rows is column n, a later row n is column half + n - (N + 1) / 2; the
  * columns between are not used. zero, uint8, lies the same way, or NULL for 8.
  * group is a power of two of at least 32 that divides K. x 16 bit [M, ldx] (dtype 0 = bf16, 1 = fp16), ldx % 8 == 0; x, codes,
  * scale and zero 16-byte aligned. y[m] = x[m] W^T (+ bias), h[m] = act(x[m] G^T) * (x[m] U^T) with G, U the first and the last
  * INTER rows of W; both contiguous. The whole number code - zero enters its product exactly, sums and scales are
- * fp32, the result is rounded once. Built for the few rows of a decode step. No counterpart in the reference, which
- * serves 8-bit weights (python/fish_scales_ops/dense/__init__.py:121-140). */
+ * fp32, the result is rounded once. The weight is read before the kernel ahead on the stream has finished: that kernel
+ * must not be the one that writes it (fso_stream_fence between the two). Built for the few rows of a decode step. No
+ * counterpart in the reference, which serves 8-bit weights (python/fish_scales_ops/dense/__init__.py:121-140). */
 int fso_int4_pack_codes(const void* codes, void* packed, int64_t n, int64_t k, void* stream);
 /* 16-bit w [N, K] -> codes, scale and (zero not NULL) zero points by rounding each group to its nearest steps: amax / 7
- * around 8, or (hi - lo) / 15 with zero inside the range; group 32, 64, 128 or 256. */
+ * around 8, or (hi - lo) / 15 with zero inside the range; group 32, 64, 128 or 256. A group that holds a NaN or an infinity
+ * gets a scale that is not a number. */
 int fso_int4_quantize(const void* w, void* codes, void* scale, void* zero, int64_t n, int64_t k, int64_t group, int64_t dtype,
                       int64_t scale_dtype, void* stream);
 int fso_int4_linear(const void* x, int64_t ldx, const void* codes, const void* scale, const void* zero, const void* bias,

@@ -10,6 +10,8 @@ pytestmark = pytest.mark.gpu
 SIZES = [(1, 32, 1, 32), (1, 128, 7, 64), (1, 4096, 100, 128), (2, 96, 65, 32), (3, 2560, 64, 128), (7, 1024, 33, 256),
          (8, 512, 130, 32), (9, 320, 257, 64), (16, 640, 48, 128), (17, 1056, 96, 32), (31, 2048, 40, 2048),
          (33, 192, 300, 64), (64, 768, 129, 128), (65, 512, 70, 128), (200, 384, 140, 64), (1, 14336, 16, 128)]
+# more tiles than SMs (whole tiles beside split ones), and than two for each; contractions off the 256-wide steps
+MANY = [(2, 1056, 10000, 32), (20, 1120, 19999, 32), (1, 320, 40010, 64), (50, 1152, 38100, 128)]
 
 
 def _linear_bound(x, w, bias=None):
@@ -27,7 +29,7 @@ def _weight(fso, n, k, group, seed, zero, scale_dtype):
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES, ids=["bf16", "fp16"])
-@pytest.mark.parametrize("t,k,n,group", SIZES)
+@pytest.mark.parametrize("t,k,n,group", SIZES + MANY)
 def test_linear(fso, device_ok, t, k, n, group, dtype):
     scale_dtype = (torch.bfloat16, torch.float16, torch.float32)[(t + n) % 3]
     weight, w = _weight(fso, n, k, group, 10 * t + n, n % 2 == 0, scale_dtype)
@@ -128,6 +130,20 @@ def test_quantized_weights_are_the_nearest_steps(fso, device_ok):
                 # half a step, and fp32 quotients that are off by a few units next to a border
                 assert ((d.view_as(v) - v).abs() <= 0.5 * step[..., None] * (1 + 1e-4)).all()
                 assert not d[3, :group].any()
+
+
+def test_quantizing_does_not_hide_a_nan(fso, device_ok):
+    for group in fso.int4.GROUP_SIZES:
+        w = R.rows(5, 512, group, torch.bfloat16, std=0.02)
+        w[1, 300] = float("nan")
+        w[3, 511] = float("-inf")
+        for zero_point in (False, True):
+            q = fso.int4.quantize_weight(w.cuda(), group_size=group, zero_point=zero_point)
+            want = torch.zeros(5, 512 // group, dtype=torch.bool)
+            want[1, 300 // group] = want[3, 511 // group] = True
+            assert torch.equal(torch.isnan(q.scale.cpu()), want)
+            y = fso.int4.linear(torch.ones(2, 512, dtype=torch.bfloat16, device="cuda"), q).cpu()
+            assert torch.equal(torch.isnan(y), torch.tensor([False, True, False, True, False]).expand(2, 5))
 
 
 def test_same_bits_every_time_and_on_another_stream(fso, device_ok):
