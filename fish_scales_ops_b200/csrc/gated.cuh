@@ -959,6 +959,42 @@ inline int make_map16(CUtensorMap* map, const void* base, int64_t rows, int64_t 
     return 0;
 }
 
+// clusters[c], c in 1..8: how many clusters of c CTAs the current device runs together with `per_sm` (1 or 2) CTAs on an SM. Fewer
+// than its SMs would hold, since those of a GPC do not divide by every c: 74, 45, 33 and 15 clusters of 2, 3, 4 and 8 on
+// 148 SMs with one, 148, 93, 71 and 33 with two. Asked once, about a stand-in with the shared memory of such CTAs: of kernels
+// that use tensor memory the driver answers for one CTA on an SM, whatever they allocate.
+__global__ void resident_clusters_kernel() {}
+
+inline int resident_clusters(int per_sm, int (&clusters)[9])
+{
+    static std::atomic<int> known[2][64][9];      // plus one
+    static std::atomic<uint64_t> done{0};
+    std::atomic<int>* const of_device = known[per_sm - 1][current_device() & 63];
+    clusters[0] = 0;
+    for (int c = 1; c <= 8; ++c) {
+        int n = of_device[c].load(std::memory_order_relaxed);
+        if (n == 0) {
+            int const rc = ensure_smem_attr(resident_clusters_kernel, 220 * 1024, done);
+            if (rc != 0) return rc;
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(static_cast<unsigned>(64 * c));
+            cfg.blockDim = dim3(256);
+            cfg.dynamicSmemBytes = per_sm == 1 ? 220 * 1024 : 110 * 1024;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = static_cast<unsigned>(c);
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            FSO_CUDA(cudaOccupancyMaxActiveClusters(&n, resident_clusters_kernel, &cfg));
+            of_device[c].store(++n, std::memory_order_relaxed);
+        }
+        clusters[c] = n - 1;
+    }
+    return 0;
+}
+
 inline int64_t gated_half_cols(int64_t inter) { return (inter + 15) / 16 * 16; }
 
 // Tiles and slices of the products. Pure host arithmetic.
@@ -984,9 +1020,13 @@ inline int forced_gated_kernel()
 // on five weights with either kernel forced: rounds of the schedule times the blocks of a slice (a 64-wide block is 512 cycles
 // at 1.55 GHz for 256 rows of x, in proportion below, 264 cycles at the least), what a tile costs beside them, and for the
 // pair kernel the traffic of split sums through L2.
-inline Gated16Plan plan_gated16_forward(int64_t t, int64_t k, int64_t inter, int sms)
+inline int plan_gated16_forward(int64_t t, int64_t k, int64_t inter, int sms, Gated16Plan& p)
 {
-    Gated16Plan p{};
+    p = Gated16Plan{};
+    int alone[9], shared[9];
+    int rc = resident_clusters(1, alone);
+    if (rc == 0) rc = resident_clusters(2, shared);
+    if (rc != 0) return rc;
     p.kb = tiles_of(k, 64);
     int const pairs = std::max(1, sms / 2);
     // few rows: token tiles of at most 256, equal, multiples of 16
@@ -994,12 +1034,13 @@ inline Gated16Plan plan_gated16_forward(int64_t t, int64_t k, int64_t inter, int
     int const n = static_cast<int>((tiles_of(t, row_tiles) + 15) / 16 * 16);
     int64_t const tiles = static_cast<int64_t>(row_tiles) * weight_tiles;
     int const slots = n <= 128 && tiles > sms ? 2 * sms : sms;
-    // Slices of at least four blocks: as many as SMs can take, at most four, each CTA with an SM to itself and its whole shared
-    // memory as a ring; a handful of tiles in eight slices (the portable cluster size), whose CTAs share SMs, because
-    // not all GPCs find eight free SMs twice.
+    // Slices of at least four blocks: at most four and as many as leave all clusters resident, each CTA with an SM to itself and
+    // its whole shared memory as a ring (36 tiles of K = 4096, one row: 9.5 us in clusters of three, 14.3 in clusters of
+    // four, of which 33 fit); a handful of tiles in eight slices (the portable cluster size), whose CTAs share SMs,
+    // because not all GPCs find eight free SMs twice.
     int const limit = n <= 128 && tiles * 8 <= sms ? 8 : 4;
     int s = 1;
-    while (s < limit && tiles * (s + 1) <= sms && (s + 1) * 4 <= p.kb) ++s;
+    while (s < limit && tiles * (s + 1) <= sms && tiles <= (s < 4 ? alone : shared)[s + 1] && (s + 1) * 4 <= p.kb) ++s;
     int const per = tiles_of(p.kb, s);
     double const rows_us = std::ceil(static_cast<double>(tiles * s) / slots) * (per * std::max(264, 2 * n) / 1550.0 * (slots > sms ? 2 : 1)
         + 2.0 + 0.035 * n) + 3.0;
@@ -1023,7 +1064,7 @@ inline Gated16Plan plan_gated16_forward(int64_t t, int64_t k, int64_t inter, int
     p.kb_per_split = rows ? per : tiles_of(p.kb, pair_s);
     p.splits = tiles_of(p.kb, p.kb_per_split);
     p.ws_bytes = !rows && p.splits > 1 ? p.splits * t * p.ws_cols * 4 : 0;
-    return p;
+    return 0;
 }
 
 // The backward pass: dx and dW share the SM pairs. Where one of them has fewer tiles than there are pairs its contraction is
@@ -1143,7 +1184,9 @@ inline int gated_forward(const void* x, int64_t ldx, const void* gate_up, void* 
     int64_t k, int64_t inter, int act, void* ws, cudaStream_t stream)
 {
     int const sms = sm_count();
-    Gated16Plan const pl = plan_gated16_forward(t, k, inter, sms);
+    Gated16Plan pl;
+    int rc = plan_gated16_forward(t, k, inter, sms, pl);
+    if (rc != 0) return rc;
     if (pl.rows_n > 0) {
         GatedRowsParams r{};
         r.t = static_cast<int>(t);
@@ -1166,7 +1209,7 @@ inline int gated_forward(const void* x, int64_t ldx, const void* gate_up, void* 
     }
     CUtensorMap m[5];
     uint16_t const* const w = static_cast<uint16_t const*>(gate_up);
-    int rc = make_map16(&m[0], x, t, k, ldx, 128);
+    rc = make_map16(&m[0], x, t, k, ldx, 128);
     if (rc == 0) rc = make_map16(&m[1], w, inter, k, k, 128);
     if (rc == 0) rc = make_map16(&m[2], w + inter * k, inter, k, k, 128);
     if (rc != 0) return rc;

@@ -578,41 +578,6 @@ inline int make_steps_map(CUtensorMap* map, const void* base, int64_t groups, in
 
 inline int64_t int4_half_cols(int64_t rows) { return ((rows + 1) / 2 + 15) / 16 * 16; }
 
-// clusters[c], c in 2..8: how many clusters of c CTAs the current device runs together, fewer than its SMs would hold, since
-// those of a GPC do not divide by every c (93, 71, 45 and 33 of 3, 4, 6 and 8 on 148 SMs). Asked once. A stand-in of the same shape is asked about: of kernels that use
-// tensor memory the driver answers for one CTA on an SM, whatever they allocate (counters show two of int4_kernel's).
-__global__ void __launch_bounds__(Int4Cfg<16>::kThreads, 2) int4_places_kernel() {}
-
-inline int int4_clusters(int (&clusters)[9])
-{
-    static std::atomic<int> known[64][9];      // plus one
-    static std::atomic<uint64_t> done{0};
-    std::atomic<int>* const of_device = known[current_device() & 63];
-    for (int c = 2; c <= 8; ++c) {
-        int n = of_device[c].load(std::memory_order_relaxed);
-        if (n == 0) {
-            constexpr int kSmem = Int4Cfg<16>::kSmemBytes;
-            int const rc = ensure_smem_attr(int4_places_kernel, kSmem, done);
-            if (rc != 0) return rc;
-            cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3(static_cast<unsigned>(64 * c));
-            cfg.blockDim = dim3(Int4Cfg<16>::kThreads);
-            cfg.dynamicSmemBytes = kSmem;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = static_cast<unsigned>(c);
-            attr[0].val.clusterDim.y = 1;
-            attr[0].val.clusterDim.z = 1;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            FSO_CUDA(cudaOccupancyMaxActiveClusters(&n, int4_places_kernel, &cfg));
-            of_device[c].store(++n, std::memory_order_relaxed);
-        }
-        clusters[c] = n - 1;
-    }
-    return 0;
-}
-
 // CTAs for `tiles` tiles on SMs that hold two CTAs each. Fewer tiles than SMs: clusters split every tile, as far as all of them
 // are resident and a slice keeps two steps (eight is the portable cluster size). 48 tiles of 16 steps take 7.0 us in 48
 // clusters of four and 10.7 in clusters of six, of which 45 fit. From there to two tiles for each SM: pairs split as
@@ -707,8 +672,8 @@ inline int launch_int4(Int4Params p, const void* x, int64_t ldx, int64_t rows, c
     maps[4] = maps[3];
     if (rc == 0 && p.has_zero) rc = make_steps_map(&maps[4], zero, groups, p.half_cols, 1, box_groups);
     if (rc != 0) return rc;
-    int clusters[9] = {};
-    rc = int4_clusters(clusters);
+    int clusters[9];
+    rc = resident_clusters(2, clusters);
     if (rc != 0) return rc;
     dim3 const grid(int4_schedule((p.rows0 + 63) / 64, sm_count(), clusters, p), static_cast<unsigned>(chunks));
     return bf16 ? launch_int4_rows<true>(n, group, maps, p, grid, stream) : launch_int4_rows<false>(n, group, maps, p, grid, stream);

@@ -696,25 +696,29 @@ int fso_gated_linear_saved_cols(int64_t inter, int64_t* cols)
 int fso_gated_linear_ws_bytes(int64_t t, int64_t k, int64_t inter, int64_t* bytes)
 {
     FSO_REQUIRE(bytes != nullptr, "fso_gated_linear_ws_bytes: bytes is NULL");
-    int const rc = check_gated_shape("fso_gated_linear_ws_bytes", t, k, inter, 0, 0);
+    int rc = check_gated_shape("fso_gated_linear_ws_bytes", t, k, inter, 0, 0);
     if (rc != 0) return rc;
-    *bytes = t == 0 ? 0 : plan_gated16_forward(t, k, inter, sm_count()).ws_bytes;
-    return 0;
+    Gated16Plan plan{};
+    if (t > 0) rc = plan_gated16_forward(t, k, inter, sm_count(), plan);
+    if (rc == 0) *bytes = plan.ws_bytes;
+    return rc;
 }
 
 int fso_gated_linear(const void* x, int64_t ldx, const void* gate_up, void* h, void* save_hi, void* save_lo, int64_t t,
     int64_t k, int64_t inter, int64_t dtype, int64_t activation, void* ws, int64_t ws_bytes, void* stream)
 {
-    int const rc = check_gated_shape("fso_gated_linear", t, k, inter, dtype, activation);
-    if (rc != 0) return rc;
-    if (t == 0) return 0;
+    int rc = check_gated_shape("fso_gated_linear", t, k, inter, dtype, activation);
+    if (rc != 0 || t == 0) return rc;
     FSO_REQUIRE(x && gate_up && h, "fso_gated_linear: NULL pointer");
     FSO_REQUIRE((save_hi == nullptr) == (save_lo == nullptr), "fso_gated_linear: save_hi and save_lo go together");
     FSO_REQUIRE(ldx >= k && ldx % 8 == 0, "fso_gated_linear: ldx = %lld must be a multiple of 8 and at least K",
         static_cast<long long>(ldx));
     FSO_REQUIRE(aligned16(x) && aligned16(gate_up) && aligned16(save_hi) && aligned16(save_lo) && aligned16(ws),
         "fso_gated_linear: x, gate_up, the saved arrays and the workspace must be 16-byte aligned");
-    int64_t const need = plan_gated16_forward(t, k, inter, sm_count()).ws_bytes;
+    Gated16Plan plan;
+    rc = plan_gated16_forward(t, k, inter, sm_count(), plan);
+    if (rc != 0) return rc;
+    int64_t const need = plan.ws_bytes;
     FSO_REQUIRE(need == 0 || (ws != nullptr && ws_bytes >= need), "fso_gated_linear: workspace of %lld bytes required, got %lld",
         static_cast<long long>(need), static_cast<long long>(ws == nullptr ? 0 : ws_bytes));
     return dtype == 0 ? gated_forward<true>(x, ldx, gate_up, h, save_hi, save_lo, t, k, inter, static_cast<int>(activation), ws, as_stream(stream))
