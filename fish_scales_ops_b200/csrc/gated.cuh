@@ -959,7 +959,7 @@ inline int make_map16(CUtensorMap* map, const void* base, int64_t rows, int64_t 
     return 0;
 }
 
-// clusters[c], c in 1..8: how many clusters of c CTAs the current device runs together with `per_sm` (1 or 2) CTAs on an SM. Fewer
+// clusters[c], c in 2..8: how many clusters of c CTAs the current device runs together with `per_sm` (1 or 2) CTAs on an SM. Fewer
 // than its SMs would hold, since those of a GPC do not divide by every c: 74, 45, 33 and 15 clusters of 2, 3, 4 and 8 on
 // 148 SMs with one, 148, 93, 71 and 33 with two. Asked once, about a stand-in with the shared memory of such CTAs: of kernels
 // that use tensor memory the driver answers for one CTA on an SM, whatever they allocate.
@@ -970,8 +970,7 @@ inline int resident_clusters(int per_sm, int (&clusters)[9])
     static std::atomic<int> known[2][64][9];      // plus one
     static std::atomic<uint64_t> done{0};
     std::atomic<int>* const of_device = known[per_sm - 1][current_device() & 63];
-    clusters[0] = 0;
-    for (int c = 1; c <= 8; ++c) {
+    for (int c = 2; c <= 8; ++c) {
         int n = of_device[c].load(std::memory_order_relaxed);
         if (n == 0) {
             int const rc = ensure_smem_attr(resident_clusters_kernel, 220 * 1024, done);
