@@ -32,6 +32,8 @@ _MAX_ROWS = 65535 * 64
 def _by_halves(t: torch.Tensor) -> torch.Tensor:
     """[N, groups] -> [groups, 2 * half], the layout the kernels read; columns between the halves are zero."""
     n, first, half = t.shape[0], (t.shape[0] + 1) // 2, _ops.int4_half_cols(t.shape[0])
+    if n == 2 * half:
+        return t.t().clone(memory_format=torch.contiguous_format)      # never the caller's memory
     out = t.new_zeros((t.shape[1], 2 * half))
     out[:, :first].copy_(t[:first].t())
     out[:, half:half + n - first].copy_(t[first:].t())

@@ -160,6 +160,20 @@ def test_same_bits_every_time_and_on_another_stream(fso, device_ok):
         assert torch.equal(first[0], fso.int4.linear(x, weight))
 
 
+def test_a_handle_has_memory_of_its_own(fso, device_ok):
+    """What the caller does to its tensors afterwards does not reach the handle, whatever their shapes."""
+    for n, groups in ((32, 1), (64, 3), (33, 1), (1, 4)):
+        codes, scale, zero = (p.cuda() for p in R.random_int4(n, 32 * groups, 32, n))
+        weight = fso.int4.prepare_weight(codes, scale, zero)
+        kept = [t.clone() for t in (codes, scale, zero)]
+        for t in (codes, scale, zero):
+            t.zero_()
+        for got, want in zip((weight.codes, weight.scale, weight.zero), kept):
+            assert torch.equal(got, want)
+        x = R.rows(2, 32 * groups, 1, torch.bfloat16).cuda()
+        R.inside(fso.int4.linear(x, weight), *_linear_bound(x, R.dequantize(*kept)))
+
+
 def test_captured_decode_steps(fso, device_ok):
     """Two captured feed-forwards (gated projection, down projection) of different sizes, replayed in turn on new inputs."""
     graphs = []
