@@ -170,11 +170,15 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
     auto dempty_bar = [&](int d) { return bars + 16u * S + 32 + 8u * d; };
     uint32_t const misc = S * C::kStageBytes + 16 * S + 48;
     // accumulators of so many units share a buffer, a wait and an arrival
-    constexpr int UB = U < C::kDCols / N ? U : C::kDCols / N;
+    constexpr int UB = U < C::kDCols / N || (N <= 32 && U * N <= 2 * C::kDCols) ? U : C::kDCols / N;
     static_assert(UB >= 1 && U % UB == 0, "batches of units");
     // The MMAs of a step fill both buffers and go on when the workers have drained one. Where that is not all of the step, the
     // workers drain it before they wait for its weights to be done with; otherwise after they have stored the next ones.
     constexpr bool kDrainFirst = U / UB > 2;
+    // One batch a step: its end is the end of the step's MMAs, so that the workers' one wait for it, before they store the next
+    // weights, answers for both, and the buffer of two steps ago is drained before they hand these over.
+    constexpr bool kOneBatch = U == UB;
+    constexpr bool kOneBuffer = UB * N > C::kDCols;      // drained before the next weights are handed over
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + misc);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(gbase + misc + 4);
 
@@ -193,7 +197,7 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(full_bar(s), 1);
-            mbar_init(empty_bar(s), C::kWorkers + 1);
+            mbar_init(empty_bar(s), kOneBatch ? 1 : C::kWorkers + 1);
         }
         mbar_init(afull_bar, C::kWorkers);
         mbar_init(aempty_bar, 1);
@@ -274,7 +278,7 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
                 uint64_t const bdesc = make_desc_sw128(base + stage * C::kStageBytes + C::kCodeBytes);
 #pragma unroll
                 for (int j = 0; j < U / UB; ++j) {
-                    if (!wait_or_abort(dempty_bar(dbuf), dphase ^ 1u, abort_flag)) {
+                    if (!kOneBatch && !wait_or_abort(dempty_bar(dbuf), dphase ^ 1u, abort_flag)) {
                         record_abort(FSO_DEV_WAIT_MMA_TMEM, abort_flag);
                         ok = false;
                         break;
@@ -287,8 +291,8 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
                         tc_mma_f16_ta(tmem + 128 + dbuf * C::kDCols + unit * N, tmem + kk * 8,
                             bdesc + static_cast<uint64_t>((kk >> 2) * (N * 128 / 16) + 2 * (kk & 3)), idesc, i % (16 / U) > 0 ? 1u : 0u);
                     }
-                    tc_commit(dfull_bar(dbuf));
-                    dbuf ^= 1;
+                    if constexpr (!kOneBatch) tc_commit(dfull_bar(dbuf));
+                    dbuf ^= kOneBuffer ? 0 : 1;
                     dphase ^= dbuf ^ 1;
                 }
                 if (!ok) break;
@@ -321,27 +325,35 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
         auto drain = [&]() -> bool {      // the units of the step before, scaled
 #pragma unroll
             for (int j = 0; j < U; j += UB) {
-                if (!wait_or_abort(dfull_bar(dbuf), dphase, abort_flag)) {
-                    if (lane == 0) record_abort(FSO_DEV_WAIT_EPILOGUE, abort_flag);
-                    return false;
+                if constexpr (!kOneBatch) {
+                    if (!wait_or_abort(dfull_bar(dbuf), dphase, abort_flag)) {
+                        if (lane == 0) record_abort(FSO_DEV_WAIT_EPILOGUE, abort_flag);
+                        return false;
+                    }
+                    __syncwarp();
+                    tc_fence_after();
                 }
-                __syncwarp();
-                tc_fence_after();
-                uint32_t r[UB * kCols];
+                constexpr int kAtOnce = kOneBuffer ? 1 : UB;      // units in registers
 #pragma unroll
-                for (int u = 0; u < UB; ++u)
+                for (int v = 0; v < UB; v += kAtOnce) {
+                    uint32_t r[kAtOnce * kCols];
 #pragma unroll
-                    for (int c = 0; c < kCols; c += 8)
-                        tmem_ld_32x8(tmem + lanes + 128 + dbuf * C::kDCols + u * N + hh * kCols + c, r + u * kCols + c);
-                tmem_ld_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(dempty_bar(dbuf));
+                    for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
-                for (int u = 0; u < UB; ++u)
+                        for (int c = 0; c < kCols; c += 8)
+                            tmem_ld_32x8(tmem + lanes + 128 + dbuf * C::kDCols + (v + u) * N + hh * kCols + c, r + u * kCols + c);
+                    tmem_ld_wait();
+                    if constexpr (!kOneBatch) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(dempty_bar(dbuf));
+                    }
 #pragma unroll
-                    for (int c = 0; c < kCols; ++c) acc[c] = fmaf(scale_now[j + u], __uint_as_float(r[u * kCols + c]), acc[c]);
-                dbuf ^= 1;
+                    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c) acc[c] = fmaf(scale_now[j + v + u], __uint_as_float(r[u * kCols + c]), acc[c]);
+                }
+                dbuf ^= kOneBuffer ? 0 : 1;
                 dphase ^= dbuf ^ 1;
             }
             return true;
@@ -394,6 +406,9 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
                     }
                     __syncwarp();
                     tc_fence_after();
+                    if constexpr (kOneBuffer) {
+                        if (st > step0) drain();
+                    }
                 }
                 tmem_st_32x32(tmem + lanes + part * 32, a);
             }
@@ -403,20 +418,28 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(afull_bar);
-                mbar_arrive(empty_bar(stage));
+                if constexpr (!kOneBatch) mbar_arrive(empty_bar(stage));
             }
             aphase ^= 1u;
             if (++stage == S) {
                 stage = 0;
                 phase ^= 1u;
             }
-            if constexpr (!kDrainFirst) {
+            if constexpr (!kDrainFirst && !kOneBuffer) {
                 if (st > step0) ok = drain();
             }
 #pragma unroll
             for (int j = 0; j < U; ++j) scale_now[j] = scale_next[j];
         }
-        if (ok && step1 > step0) ok = drain();
+        if (ok && step1 > step0) {
+            if (kOneBatch && !wait_or_abort(aempty_bar, aphase ^ 1u, abort_flag)) {
+                if (lane == 0) record_abort(FSO_DEV_WAIT_EPILOGUE, abort_flag);
+                ok = false;
+            }
+            __syncwarp();
+            tc_fence_after();
+            if (ok) ok = drain();
+        }
         // every MMA and every copy is done: the sums of this slice go where the stages were
         asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kWorkers) : "memory");
         if (ok) {
