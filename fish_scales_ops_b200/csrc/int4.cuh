@@ -62,6 +62,13 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t saddr)
     return v;
 }
 
+__device__ __forceinline__ uint32_t lds_u32(uint32_t saddr)
+{
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(saddr) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ uint32_t lds_u8(uint32_t saddr)
 {
     uint32_t v;
@@ -368,12 +375,25 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
             }
             __syncwarp();
             uint32_t const src = base + stage * C::kStageBytes;
+            // By branches that the whole grid takes alike up to 32 rows (one row on 28672 x 4096: 17.8 us, 18.5 without); beyond, where
+            // registers are short, both halves of an fp32 scale are read always (48 rows: 25.6 us, 26.3 with branches).
+            if constexpr (N > 32) {
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                uint32_t const at = src + scale_row + (j & unit_mask) * 64 * scale_width;
-                uint32_t const upper = lds_u16(at + scale_width - 2), lower = lds_u16(at);
-                scale_next[j] = p.scale_type == 1 ? __half2float(__ushort_as_half(static_cast<uint16_t>(upper)))
-                                                  : __uint_as_float(upper << 16 | (p.scale_type == 2 ? lower : 0u));
+                for (int j = 0; j < U; ++j) {
+                    uint32_t const at = src + scale_row + (j & unit_mask) * 64 * scale_width;
+                    uint32_t const upper = lds_u16(at + scale_width - 2), lower = lds_u16(at);
+                    scale_next[j] = p.scale_type == 1 ? __half2float(__ushort_as_half(static_cast<uint16_t>(upper)))
+                                                      : __uint_as_float(upper << 16 | (p.scale_type == 2 ? lower : 0u));
+                }
+            } else if (p.scale_type == 2) {
+#pragma unroll
+                for (int j = 0; j < U; ++j) scale_next[j] = __uint_as_float(lds_u32(src + scale_row + (j & unit_mask) * 256));
+            } else {
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    uint32_t const v = lds_u16(src + scale_row + (j & unit_mask) * 128);
+                    scale_next[j] = p.scale_type == 1 ? __half2float(__ushort_as_half(static_cast<uint16_t>(v))) : __uint_as_float(v << 16);
+                }
             }
 #pragma unroll
             for (int b = 0; b < 2; ++b) {      // 64 of the contraction
@@ -385,8 +405,14 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
 #pragma unroll
                 for (int q = 0; q < kZeros; ++q) {
                     int const j = U == 8 ? 2 * part + q : U == 4 ? part : part >> 1;
-                    uint32_t const z = lds_u8(src + zero_row + (j & unit_mask) * 64);
-                    zero2[q] = ((kBf16 ? 0x4300u : 0x6400u) + (p.has_zero ? z : 8u)) * 0x10001u;
+                    uint32_t z = 8u;
+                    if constexpr (N > 16) {
+                        uint32_t const stored = lds_u8(src + zero_row + (j & unit_mask) * 64);
+                        z = p.has_zero ? stored : 8u;
+                    } else {
+                        if (p.has_zero) z = lds_u8(src + zero_row + (j & unit_mask) * 64);
+                    }
+                    zero2[q] = (kBf16 ? 0x43004300u : 0x64006400u) + z * 0x10001u;
                 }
                 uint32_t a[32];
                 uint32_t const words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
