@@ -34,31 +34,53 @@ struct Int4Params {
     int steps_per_slice;
 };
 
-// Eight codes of a word to the eight 16-bit numbers code - zero, exactly: a code in the low bits of the mantissa of 128
-// (bf16) or 1024 (fp16) is 128 + code, and taking away 128 + zero is exact. Register i gets k = 2 i and 2 i + 1 of the
-// word. The ten bits of fp16 hold the next code as well, as 1024 + 16 code, and a sixteenth of that less 64 + zero is exact too:
-// one shift instead of three. `zero2` is the first minuend twice, `zero16` the second (fp16).
+// Eight codes of a word to the eight 16-bit numbers code - zero (bf16: a 64th of that), exactly, with one shift, four masks and
+// four multiply-adds; register i gets k = 2 i and 2 i + 1 of the word.
+//
+// fp16: a code in the low bits of the mantissa of 1024 is 1024 + code, the next one in the ten bits 1024 + 16 code; the first
+// less 1024 + zero, and a sixteenth of the second less 64 + zero, are exact.
+// bf16 has seven bits of mantissa, too few for two codes. But the bits of the smallest numbers are linear across the border of
+// normal ones: the lower eight bits alone, read as bf16, are that whole number times 2^-133. Times 2^127 (the second code, which
+// stands 16 times higher, times 2^123) and less zero / 64 it is (code - zero) / 64; the 64 comes back with the sums.
+constexpr float kInt4Unit = 64.f;
+
 template <bool kBf16>
-__device__ __forceinline__ void int4_unpack(uint32_t w, uint32_t zero2, uint32_t zero16, uint32_t* r)
-{
-    if constexpr (kBf16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t v;
-            asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w >> (4 * i)), "n"(0x000F000F), "n"(0x43004300));      // (a & b) | c
-            __nv_bfloat162 const d = __hsub2(*reinterpret_cast<__nv_bfloat162 const*>(&v), *reinterpret_cast<__nv_bfloat162 const*>(&zero2));
-            r[i] = *reinterpret_cast<uint32_t const*>(&d);
+struct Int4Zero {
+    uint32_t first, second;      // what is taken away from either, twice
+
+    __device__ __forceinline__ void set(uint32_t z)
+    {
+        if constexpr (kBf16) {
+            uint32_t const bits = z * 0x10001u, scale = 0x7F007F00u;
+            __nv_bfloat162 const v = __hmul2(*reinterpret_cast<__nv_bfloat162 const*>(&bits), *reinterpret_cast<__nv_bfloat162 const*>(&scale));
+            first = second = *reinterpret_cast<uint32_t const*>(&v);
+        } else {
+            first = 0x64006400u + z * 0x10001u;        // 1024 + zero
+            second = 0x54005400u + z * 0x100010u;      // 64 + zero
         }
-    } else {
+    }
+};
+
+template <bool kBf16>
+__device__ __forceinline__ void int4_unpack(uint32_t w, Int4Zero<kBf16> const& zero, uint32_t* r)
+{
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            uint32_t const at = w >> (4 * i);
+    for (int i = 0; i < 4; i += 2) {
+        uint32_t const at = w >> (4 * i);
+        if constexpr (kBf16) {
+            uint32_t const lo = at & 0x000F000Fu, hi = at & 0x00F000F0u, m0 = 0x7F007F00u, m1 = 0x7D007D00u;      // 2^127, 2^123
+            __nv_bfloat162 const z = __hneg2(*reinterpret_cast<__nv_bfloat162 const*>(&zero.first));
+            __nv_bfloat162 const d = __hfma2(*reinterpret_cast<__nv_bfloat162 const*>(&lo), *reinterpret_cast<__nv_bfloat162 const*>(&m0), z);
+            __nv_bfloat162 const e = __hfma2(*reinterpret_cast<__nv_bfloat162 const*>(&hi), *reinterpret_cast<__nv_bfloat162 const*>(&m1), z);
+            r[i] = *reinterpret_cast<uint32_t const*>(&d);
+            r[i + 1] = *reinterpret_cast<uint32_t const*>(&e);
+        } else {
             uint32_t lo, hi;
-            asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(lo) : "r"(at), "n"(0x000F000F), "n"(0x64006400));
+            asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(lo) : "r"(at), "n"(0x000F000F), "n"(0x64006400));      // (a & b) | c
             asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(hi) : "r"(at), "n"(0x00F000F0), "n"(0x64006400));
-            __half2 const d = __hsub2(*reinterpret_cast<__half2 const*>(&lo), *reinterpret_cast<__half2 const*>(&zero2));
+            __half2 const d = __hsub2(*reinterpret_cast<__half2 const*>(&lo), *reinterpret_cast<__half2 const*>(&zero.first));
             __half2 const e = __hfma2(*reinterpret_cast<__half2 const*>(&hi), __float2half2_rn(0.0625f),
-                __hneg2(*reinterpret_cast<__half2 const*>(&zero16)));
+                __hneg2(*reinterpret_cast<__half2 const*>(&zero.second)));
             r[i] = *reinterpret_cast<uint32_t const*>(&d);
             r[i + 1] = *reinterpret_cast<uint32_t const*>(&e);
         }
@@ -411,7 +433,7 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
                 uint4 const c0 = lds_v4(src + code_row + (((2 * part) ^ (in_half & 7)) << 4));
                 uint4 const c1 = lds_v4(src + code_row + (((2 * part + 1) ^ (in_half & 7)) << 4));
                 constexpr int kZeros = U == 8 ? 2 : 1;      // groups of these 64
-                uint32_t zero2[kZeros], zero16[kZeros];
+                Int4Zero<kBf16> zero[kZeros];
 #pragma unroll
                 for (int q = 0; q < kZeros; ++q) {
                     int const j = U == 8 ? 2 * part + q : U == 4 ? part : part >> 1;
@@ -422,13 +444,12 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
                     } else {
                         if (p.has_zero) z = lds_u8(src + zero_row + (j & unit_mask) * 64);
                     }
-                    zero2[q] = (kBf16 ? 0x43004300u : 0x64006400u) + z * 0x10001u;
-                    zero16[q] = 0x54005400u + z * 0x100010u;      // 64 + zero in fp16
+                    zero[q].set(z);
                 }
                 uint32_t a[32];
                 uint32_t const words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-                for (int j = 0; j < 8; ++j) int4_unpack<kBf16>(words[j], zero2[j * kZeros >> 3], zero16[j * kZeros >> 3], a + 4 * j);
+                for (int j = 0; j < 8; ++j) int4_unpack<kBf16>(words[j], zero[j * kZeros >> 3], a + 4 * j);
                 if (b == 0) {
                     if constexpr (kDrainFirst) {
                         if (st > step0 && !drain()) {
@@ -482,7 +503,7 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
         if (ok) {
             float* const red = reinterpret_cast<float*>(gbase);
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) red[(hh * kCols + c) * C::kRedStride + row] = acc[c];
+            for (int c = 0; c < kCols; ++c) red[(hh * kCols + c) * C::kRedStride + row] = kBf16 ? kInt4Unit * acc[c] : acc[c];
         }
     }
     __syncthreads();
