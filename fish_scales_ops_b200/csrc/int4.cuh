@@ -427,29 +427,29 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
                     scale_next[j] = p.scale_type == 1 ? __half2float(__ushort_as_half(static_cast<uint16_t>(v))) : __uint_as_float(v << 16);
                 }
             }
+            constexpr int kZeros = U / 2;      // groups of this worker's 128
+            Int4Zero<kBf16> zero[kZeros];
+#pragma unroll
+            for (int q = 0; q < kZeros; ++q) {
+                uint32_t const at = src + zero_row + ((hh * kZeros + q) & unit_mask) * 64;
+                uint32_t z = 8u;
+                if constexpr (N > 16) {
+                    uint32_t const stored = lds_u8(at);
+                    z = p.has_zero ? stored : 8u;
+                } else {
+                    if (p.has_zero) z = lds_u8(at);
+                }
+                zero[q].set(z);
+            }
 #pragma unroll
             for (int b = 0; b < 2; ++b) {      // 64 of the contraction
                 int const part = 2 * hh + b;
                 uint4 const c0 = lds_v4(src + code_row + (((2 * part) ^ (in_half & 7)) << 4));
                 uint4 const c1 = lds_v4(src + code_row + (((2 * part + 1) ^ (in_half & 7)) << 4));
-                constexpr int kZeros = U == 8 ? 2 : 1;      // groups of these 64
-                Int4Zero<kBf16> zero[kZeros];
-#pragma unroll
-                for (int q = 0; q < kZeros; ++q) {
-                    int const j = U == 8 ? 2 * part + q : U == 4 ? part : part >> 1;
-                    uint32_t z = 8u;
-                    if constexpr (N > 16) {
-                        uint32_t const stored = lds_u8(src + zero_row + (j & unit_mask) * 64);
-                        z = p.has_zero ? stored : 8u;
-                    } else {
-                        if (p.has_zero) z = lds_u8(src + zero_row + (j & unit_mask) * 64);
-                    }
-                    zero[q].set(z);
-                }
                 uint32_t a[32];
                 uint32_t const words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-                for (int j = 0; j < 8; ++j) int4_unpack<kBf16>(words[j], zero[j * kZeros >> 3], a + 4 * j);
+                for (int j = 0; j < 8; ++j) int4_unpack<kBf16>(words[j], zero[(8 * b + j) * kZeros >> 4], a + 4 * j);
                 if (b == 0) {
                     if constexpr (kDrainFirst) {
                         if (st > step0 && !drain()) {
