@@ -178,14 +178,14 @@ struct Int4Cfg {
 //
 // The weight bytes are the bound, so they are streamed by TMA, about 100 KB of an SM's on their way, and what has to be done to
 // a weight is kept below the time that its half byte takes: a worker reads 32 codes with one load, turns a word of
-// eight into four registers with eleven instructions and stores them to tensor memory, where the MMA (kind::f16)
-// takes its A operand from; with A in shared memory the same MMA takes 40 cycles instead of 10 (N = 16), more than the
+// eight into four registers with nine instructions (with eleven, three of them shifts, one row on 28672 x 4096 takes
+// 17.8 us instead of 16.0) and stores them to tensor memory, where the MMA (kind::f16) takes its A operand from; with A in shared memory the same MMA takes 40 cycles instead of 10 (N = 16), more than the
 // bytes do. Every group has an accumulator of its own, which the workers scale in fp32 into their registers. The CTAs
 // of a cluster split the contraction of a tile where tiles are few or do not come out even, and each adds up a part of
 // the outputs over distributed shared memory, in a fixed order.
 //
-// What a step costs beside the unpacking (three waits, three arrivals, addresses: about a hundred instructions of a warp)
-// is paid once for 256 of the contraction; one buffer of unpacked weights is enough, since the MMAs of a step take less than
+// What a step costs beside the unpacking (waits, arrivals, scales, addresses: as many instructions as the unpacking itself)
+// is paid once for 256 of the contraction, 0.93 us for two CTAs of an SM; one buffer of unpacked weights is enough, since the MMAs of a step take less than
 // the unpacking of the next.
 //
 // U: units of a step that have sums of their own: its groups, or two halves of 128 where a group is longer.
@@ -211,10 +211,10 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
     // accumulators of so many units share a buffer, a wait and an arrival
     constexpr int UB = U < C::kDCols / N || (N <= 32 && U * N <= 2 * C::kDCols) ? U : C::kDCols / N;
     static_assert(UB >= 1 && U % UB == 0, "batches of units");
-    // The MMAs of a step fill both buffers and go on when the workers have drained one. Where that is not all of the step, the
+    // More than one batch: the MMAs of a step fill both buffers and go on when the workers have drained one. Where that is not all of the step, the
     // workers drain it before they wait for its weights to be done with; otherwise after they have stored the next ones.
     constexpr bool kDrainFirst = U / UB > 2;
-    // One batch a step: its end is the end of the step's MMAs, so that the workers' one wait for it, before they store the next
+    // One batch a step (up to 32 rows; with more, one buffer for it takes 4 % more time than two batches): its end is the end of the step's MMAs, so that the workers' one wait for it, before they store the next
     // weights, answers for both, and the buffer of two steps ago is drained before they hand these over.
     constexpr bool kOneBatch = U == UB;
     constexpr bool kOneBuffer = UB * N > C::kDCols;      // drained before the next weights are handed over
@@ -407,8 +407,8 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
             }
             __syncwarp();
             uint32_t const src = base + stage * C::kStageBytes;
-            // By branches that the whole grid takes alike up to 32 rows (one row on 28672 x 4096: 17.8 us, 18.5 without); beyond, where
-            // registers are short, both halves of an fp32 scale are read always (48 rows: 25.6 us, 26.3 with branches).
+            // By branches that the whole grid takes alike up to 32 rows (one row on 28672 x 4096: 4 % less time); beyond, where
+            // registers are short, both halves of an fp32 scale are read always (48 rows: 3 % less time than with branches).
             if constexpr (N > 32) {
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
@@ -660,8 +660,8 @@ inline int make_steps_map(CUtensorMap* map, const void* base, int64_t groups, in
 inline int64_t int4_half_cols(int64_t rows) { return ((rows + 1) / 2 + 15) / 16 * 16; }
 
 // CTAs for `tiles` tiles on SMs that hold two CTAs each. Fewer tiles than SMs: clusters split every tile, as far as all of them
-// are resident and a slice keeps two steps (eight is the portable cluster size). 48 tiles of 16 steps take 7.0 us in 48
-// clusters of four and 10.7 in clusters of six, of which 45 fit. From there to two tiles for each SM: pairs split as
+// are resident and a slice keeps two steps (eight is the portable cluster size). 48 tiles of 16 steps take a third
+// less time in 48 clusters of four (6.3 us) than in clusters of six, of which 45 fit. From there to two tiles for each SM: pairs split as
 // many tiles as fill the places that one CTA for each tile would leave. More: the last tiles are split, so that the
 // end of the last round is short.
 inline unsigned int4_schedule(int tiles, int sms, int const (&clusters)[9], Int4Params& p)
