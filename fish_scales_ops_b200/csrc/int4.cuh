@@ -211,11 +211,13 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
     // accumulators of so many units share a buffer, a wait and an arrival
     constexpr int UB = U < C::kDCols / N || (N <= 32 && U * N <= 2 * C::kDCols) ? U : C::kDCols / N;
     static_assert(UB >= 1 && U % UB == 0, "batches of units");
-    // More than one batch: the MMAs of a step fill both buffers and go on when the workers have drained one. Where that is not all of the step, the
-    // workers drain it before they wait for its weights to be done with; otherwise after they have stored the next ones.
+    // More than one batch: the MMAs of a step fill both buffers and go on when the workers have drained one. Where that is not all
+    // of the step, the workers drain it before they wait for its weights to be done with; otherwise after they have
+    // stored the next ones.
     constexpr bool kDrainFirst = U / UB > 2;
-    // One batch a step (up to 32 rows; with more, one buffer for it takes 4 % more time than two batches): its end is the end of the step's MMAs, so that the workers' one wait for it, before they store the next
-    // weights, answers for both, and the buffer of two steps ago is drained before they hand these over.
+    // One batch a step (up to 32 rows; with more, one buffer for it takes 4 % more time than two batches): its end is the end of
+    // the step's MMAs, so that the workers' one wait for it, before they store the next weights, answers for both, and the
+    // buffer of two steps ago is drained before they hand these over.
     constexpr bool kOneBatch = U == UB;
     constexpr bool kOneBuffer = UB * N > C::kDCols;      // drained before the next weights are handed over
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + misc);

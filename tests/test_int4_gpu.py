@@ -113,6 +113,14 @@ def test_extreme_values_stay_in_their_row(fso, device_ok):
     assert torch.equal(torch.nan_to_num(got[11], nan=7.0), torch.nan_to_num(inf, nan=7.0))
 
 
+@pytest.mark.parametrize("power", [-126, -116, 100, 116])
+def test_rows_of_any_magnitude(fso, device_ok, power):
+    """bf16 rows around the smallest normal numbers and near the largest: the same bound as everywhere."""
+    weight, w = _weight(fso, 64, 256, 64, 3, True, torch.float32)
+    x = (R.rows(4, 256, 1, torch.float32) * 2.0 ** power).to(torch.bfloat16).cuda()
+    R.inside(fso.int4.linear(x, weight), *_linear_bound(x, w))
+
+
 def test_quantized_weights_are_the_nearest_steps(fso, device_ok):
     for dtype in R.DTYPES:
         for group in fso.int4.GROUP_SIZES:
