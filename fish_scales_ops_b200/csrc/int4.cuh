@@ -266,7 +266,7 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
             int const row0 = tile * 64;
             int const box_groups = max(1, C::kStep >> p.group_shift);
             uint32_t const scale_bytes = box_groups * 64 * (p.scale_type == 2 ? 4 : 2), zero_bytes = box_groups * 64;
-            uint32_t const bytes = C::kCodeBytes + C::kXBytes + 2 * scale_bytes + (p.has_zero ? 2 * zero_bytes : 0);
+            uint32_t const bytes = C::kCodeBytes + p.chunk_rows * (C::kStep * 2) + 2 * scale_bytes + (p.has_zero ? 2 * zero_bytes : 0);
             auto load_weight = [&](int stage, int st) {
                 uint32_t const fb = full_bar(stage), dst = base + stage * C::kStageBytes;
                 int const g0 = (st * C::kStep) >> p.group_shift;
@@ -750,7 +750,9 @@ inline int launch_int4(Int4Params p, const void* x, int64_t ldx, int64_t rows, c
     int rc = make_codes_map(&maps[0], c, p.rows0, p.k);
     maps[1] = maps[0];      // a weight of one row has no second half: what is read in its place goes nowhere
     if (rc == 0 && p.rows1 > 0) rc = make_codes_map(&maps[1], c + static_cast<int64_t>(p.rows0) * (p.k / 2), p.rows1, p.k);
-    if (rc == 0) rc = make_map16(&maps[2], x, p.m, p.k, ldx, n);
+    // x in boxes of as many rows as there are: to fill the rest of a tile with zeros costs TMA time (one row on 28672 x 4096: 15.0
+    // us, 16.0 with 15 rows of zeros). What lies in its place goes into sums that nobody reads.
+    if (rc == 0) rc = make_map16(&maps[2], x, p.m, p.k, ldx, p.chunk_rows);
     if (rc == 0) rc = make_steps_map(&maps[3], scale, groups, p.half_cols, p.scale_type == 2 ? 4 : 2, box_groups);
     maps[4] = maps[3];
     if (rc == 0 && p.has_zero) rc = make_steps_map(&maps[4], zero, groups, p.half_cols, 1, box_groups);
