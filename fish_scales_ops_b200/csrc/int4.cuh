@@ -152,17 +152,18 @@ __device__ __forceinline__ void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, 
         : "memory");
 }
 
-template <int N>
+template <int N, int U>
 struct Int4Cfg {
     static constexpr int kWorkers = 8;                   // warps that unpack and drain
     static constexpr int kThreads = 64 + 32 * kWorkers;  // TMA, MMA, workers
     static constexpr int kStep = 256;                    // of the contraction in a stage
     static constexpr int kCodeBytes = 128 * kStep / 2;
     static constexpr int kXBytes = N * kStep * 2;        // four tiles of N rows x 64 elements
-    static constexpr int kScaleOff = kCodeBytes + kXBytes;       // [half][group][64 rows], at most eight groups
-    static constexpr int kZeroOff = kScaleOff + 2 * 8 * 64 * 4;
-    static constexpr int kStageBytes = (kZeroOff + 2 * 8 * 64 + 1023) / 1024 * 1024;
-    static constexpr int kStages = (109 * 1024) / kStageBytes;
+    static constexpr int kScaleOff = kCodeBytes + kXBytes;       // [half][group][64 rows], of at most 4 bytes
+    static constexpr int kZeroOff = kScaleOff + 2 * U * 64 * 4;
+    static constexpr int kStageBytes = (kZeroOff + 2 * U * 64 + 1023) / 1024 * 1024;
+    // up to three: a fourth, where it fits, saves one row 2 % on 28672 x 4096 and costs it 5 % on 4096 x 14336
+    static constexpr int kStages = (109 * 1024) / kStageBytes < 3 ? (109 * 1024) / kStageBytes : 3;
     static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 512;
     // tensor memory: the unpacked weights of a step (256 elements, 128 columns), then two buffers of group accumulators
     static constexpr int kDCols = 64;
@@ -190,12 +191,12 @@ struct Int4Cfg {
 //
 // U: units of a step that have sums of their own: its groups, or two halves of 128 where a group is longer.
 template <bool kBf16, int N, int U>
-__global__ void __launch_bounds__(Int4Cfg<N>::kThreads, 2)
+__global__ void __launch_bounds__(Int4Cfg<N, U>::kThreads, 2)
 int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ CUtensorMap tm_hi,
     const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_scale, const __grid_constant__ CUtensorMap tm_zero,
     const Int4Params p)
 {
-    using C = Int4Cfg<N>;
+    using C = Int4Cfg<N, U>;
     constexpr int S = C::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint32_t const raw = smem_u32(smem_raw);
@@ -275,8 +276,8 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
                 tma_load_2d(dst + 8192, &tm_hi, fb, st * (C::kStep / 2), row0);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    tma_load_2d(dst + C::kScaleOff + h * 2048, &tm_scale, fb, row0 + h * p.half_cols, g0);
-                    if (p.has_zero) tma_load_2d(dst + C::kZeroOff + h * 512, &tm_zero, fb, row0 + h * p.half_cols, g0);
+                    tma_load_2d(dst + C::kScaleOff + h * (U * 256), &tm_scale, fb, row0 + h * p.half_cols, g0);
+                    if (p.has_zero) tma_load_2d(dst + C::kZeroOff + h * (U * 64), &tm_zero, fb, row0 + h * p.half_cols, g0);
                 }
             };
             auto load_x = [&](int stage, int st) {
@@ -355,7 +356,7 @@ int4_kernel(const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ C
         uint32_t const lanes = static_cast<uint32_t>(quarter * 32) << 16;
         uint32_t const code_row = half * 8192 + in_half * 128;
         uint32_t const scale_width = p.scale_type == 2 ? 4 : 2;
-        uint32_t const scale_row = C::kScaleOff + half * 2048 + in_half * scale_width, zero_row = C::kZeroOff + half * 512 + in_half;
+        uint32_t const scale_row = C::kScaleOff + half * (U * 256) + in_half * scale_width, zero_row = C::kZeroOff + half * (U * 64) + in_half;
         int const unit_mask = U == 2 && p.group_shift >= 8 ? 0 : U - 1;      // units that share a longer group
         constexpr int kCols = N / 2;
         float acc[kCols] = {};
@@ -691,7 +692,7 @@ inline unsigned int4_schedule(int tiles, int sms, int const (&clusters)[9], Int4
 template <bool kBf16, int N, int U>
 inline int launch_int4_inst(CUtensorMap const (&maps)[5], Int4Params const& p, dim3 grid, cudaStream_t stream)
 {
-    using C = Int4Cfg<N>;
+    using C = Int4Cfg<N, U>;
     static std::atomic<uint64_t> done{0};
     auto kernel = int4_kernel<kBf16, N, U>;
     int const rc = ensure_smem_attr(kernel, C::kSmemBytes, done);
