@@ -180,14 +180,16 @@ struct Int4Cfg {
 // The weight bytes are the bound, so they are streamed by TMA, about 100 KB of an SM's on their way, and what has to be done to
 // a weight is kept below the time that its half byte takes: a worker reads 32 codes with one load, turns a word of
 // eight into four registers with nine instructions (with eleven, three of them shifts, one row on 28672 x 4096 takes
-// 17.8 us instead of 16.0) and stores them to tensor memory, where the MMA (kind::f16) takes its A operand from; with A in shared memory the same MMA takes 40 cycles instead of 10 (N = 16), more than the
-// bytes do. Every group has an accumulator of its own, which the workers scale in fp32 into their registers. The CTAs
-// of a cluster split the contraction of a tile where tiles are few or do not come out even, and each adds up a part of
-// the outputs over distributed shared memory, in a fixed order.
+// 17.8 us instead of 16.0) and stores them to tensor memory, where the MMA (kind::f16) takes its A operand from; with A in
+// shared memory the same MMA takes 40 cycles instead of 10 (N = 16), more than the bytes do. Every group has an accumulator of
+// its own, which the workers scale in fp32 into their registers. The CTAs of a cluster split the contraction of a tile
+// where tiles are few or do not come out even, and each adds up a part of the outputs over distributed shared memory, in
+// a fixed order.
 //
 // What a step costs beside the unpacking (waits, arrivals, scales, addresses: as many instructions as the unpacking itself)
-// is paid once for 256 of the contraction, 0.93 us for two CTAs of an SM; one buffer of unpacked weights is enough, since the MMAs of a step take less than
-// the unpacking of the next.
+// is paid once for 256 of the contraction, 0.9 us for two CTAs of an SM; one buffer of unpacked weights is enough, since the
+// MMAs of a step take less than the unpacking of the next. 28672 x 4096, groups of 128 with zero points: 14.9 us for one
+// row (4.1 TB/s), 17.0 for 20 (groups of 64: 16.7 for 16), 24.1 for 48, 37888 x 8192 29.4 (5.5 TB/s).
 //
 // U: units of a step that have sums of their own: its groups, or two halves of 128 where a group is longer.
 template <bool kBf16, int N, int U>
